@@ -436,6 +436,113 @@ int mf_prefill_attention_tc(void* out_hi, void* out_lo, const float* q, const vo
                             int max_seq, int n_tokens, int pos0, int n_heads, int n_kv_heads, int d_head,
                             void* scratch, size_t scratch_bytes, int kv_dtype, void* stream);
 /* ===================================================================== */
+/* One step of a batch of sequences over a paged KV cache                 */
+/* ===================================================================== */
+/* No reference counterpart: the reference keeps one contiguous cache for one
+ * sequence (src/base/config.cpp:362-363). Here a layer's K and V rows live in
+ * pages of page_size positions that a table assigns to sequences, and a call
+ * works on the new tokens of all sequences at once: rows
+ * [q_start[b], q_start[b + 1]) of the call are the last tokens of sequence b,
+ * whose length with them is kv_lens[b] (token i of n_b has position
+ * kv_lens[b] - n_b + i). Rows outside [q_start[0], q_start[n_seqs]) belong to
+ * nobody and their outputs are left as they were.
+ *
+ * q_start, kv_lens and the table are device arrays, read by the kernels only,
+ * so a captured launch serves changing batches. q_start must not decrease.
+ * Nothing in them can make a kernel leave its buffers: starts are clamped to
+ * the call's rows, lengths to max_pages * page_size, and a page id outside
+ * [0, n_pages) holds no keys: nothing is appended there, and its positions
+ * are as if masked (a scheduler may so drop whole pages, e.g. behind a
+ * window). A token before position 0 (kv_lens[b] < n_b) appends nothing and
+ * sees nothing. */
+typedef struct mf_paged_kv {
+    void* k_pages; /* element (page, head, row, d) at page * page_stride + head * head_stride + row * row_stride + d */
+    void* v_pages;
+    long long page_stride; /* elements; 0: n_kv_heads * head_stride */
+    long long head_stride; /* 0: page_size * d_head */
+    long long row_stride;  /* 0: d_head. All multiples of 16 bytes, the pages 16-byte aligned */
+    const int* page_table; /* [n_seqs][table_stride], the first max_pages of each row */
+    const int* q_start;    /* [n_seqs + 1] */
+    const int* kv_lens;    /* [n_seqs] */
+    int table_stride;      /* 0: max_pages */
+    int max_pages;
+    int n_pages;
+    int page_size; /* a multiple of 8 */
+    int n_seqs;
+    int n_kv_heads;
+    int d_head; /* 64 or 128 */
+    int dtype;  /* of the pages, and of q_out, q and out */
+} mf_paged_kv;
+
+/* Host helper: rotary frequencies of mf_paged_rope_append, out[j] in turns per
+ * position for the d_rot / 2 pairs, and the magnitude of the rotation
+ * (*mscale; 1 except for MF_ROPE_YARN). Plain: base^(-2j/d_rot) / (2 pi).
+ * Linear: divided by factor. NTK: base * factor^(d_rot / (d_rot - 2)) in place
+ * of base. YaRN (as published): pairs that turn more than beta_fast times over
+ * orig_ctx positions keep their frequency, those below beta_slow turns are
+ * divided by factor, a linear ramp between; mscale = 0.1 ln(factor) + 1. */
+#define MF_ROPE_PLAIN 0
+#define MF_ROPE_LINEAR 1
+#define MF_ROPE_NTK 2
+#define MF_ROPE_YARN 3
+int mf_rope_freqs(double* out, int d_rot, double base, int scaling, double factor, double orig_ctx, double beta_fast,
+                  double beta_slow, float* mscale);
+
+/* Q/K RMSNorm (optional), rotary positions and the append of all new tokens
+ * (what mf_prefill_qkv_post does for one sequence; src/models/qwen3/
+ * module.cpp:193-226, src/ops/kernels.cpp:31-82): the rotated q heads go to
+ * q_out, k and v to their page rows, rounded to the pages' type. The first
+ * d_rot elements of a head are rotated in pairs (j, j + d_rot / 2), or
+ * (2j, 2j + 1) with `interleaved`; the others pass through. Angles are reduced
+ * in 64 bits, so far positions are as exact as near ones. */
+typedef struct mf_paged_rope_desc {
+    void* q_out;        /* [n_tokens][q_stride], n_heads * d_head of each row */
+    long long q_stride; /* elements; 0: n_heads * d_head */
+    const void* qkv;    /* [n_tokens][x_stride]: q heads, k heads, v heads */
+    long long x_stride; /* 0: (n_heads + 2 n_kv_heads) * d_head */
+    int x_dtype;
+    int n_tokens;
+    int n_heads;
+    int d_rot; /* a multiple of 8, 0 .. d_head */
+    int interleaved;
+    float mscale;
+    float eps;
+    const double* freqs;    /* [d_rot / 2], device (mf_rope_freqs); NULL for d_rot 0 */
+    const float* q_norm_w;  /* [d_head] or NULL: no norm */
+    const float* k_norm_w;
+    const int* positions;   /* [n_tokens] rotary positions, or NULL: the cache positions */
+} mf_paged_rope_desc;
+int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* desc, void* stream);
+
+/* Attention of the new tokens over the cached positions, their own included:
+ * softmax over the positions s with pos - window < s <= pos (window 0: all up
+ * to pos) of scale * q.k_s, times v_s; query heads share KV head h / G. A row
+ * that sees no position is 0. Positions that no row of the call sees are never
+ * used, whatever their pages hold; a position that some rows of a sequence see
+ * must hold finite values (it may enter the others' sums with weight 0).
+ * max_new and max_len (0: unknown) are hints, the largest n_b and kv_lens[b]:
+ * they choose between kernels, never what is computed. The workspace
+ * (mf_paged_attention_workspace_bytes, 256-byte aligned) needs no
+ * initialisation and holds nothing after the call; calls that overlap on the
+ * GPU need workspaces of their own. */
+typedef struct mf_paged_attn_desc {
+    void* out;            /* [n_tokens][out_stride] */
+    long long out_stride; /* elements; 0: n_heads * d_head */
+    const void* q;        /* [n_tokens][q_stride] */
+    long long q_stride;
+    int n_tokens;
+    int n_heads;
+    float scale; /* 0: 1 / sqrt(d_head) */
+    int window;
+    int max_new;
+    int max_len;
+    void* workspace;
+    size_t workspace_bytes;
+} mf_paged_attn_desc;
+size_t mf_paged_attention_workspace_bytes(int n_tokens, int n_heads, int n_kv_heads, int d_head, int dtype);
+int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* desc, void* stream);
+
+/* ===================================================================== */
 /* Sampling on the device                                                */
 /* ===================================================================== */
 /* The k (<= 64) largest of x[0, n) and their indices, sorted by value,
@@ -458,6 +565,21 @@ int mf_topk(const float* x, int n, int k, int* ids, float* vals, void* workspace
  * candidate filtered out. No presence penalty (it changes the list). */
 int mf_sample_step(const int* cand_ids, const float* cand_vals, int top_k, float temp, float top_p, float min_p,
                    const float* draws, int n_draws, void* step_state, int* out_ids, int* flags, void* stream);
+
+/* One id per row of logits [n_rows][ld] (dtype MF_F32, MF_F16 or MF_BF16), each
+ * row with its own parameters and random number (device arrays): the filters
+ * of Sampler::sample in its order (src/base/sampler.cpp:40-117) over the
+ * candidates sorted by value, equal values by index, NaN as -inf: the top_k
+ * first (<= 0 or >= vocab: all), the shortest prefix with softmax mass top_p
+ * (>= 1: all), those with x >= top + log(min_p) (<= 0: all), then the first
+ * whose cumulative softmax(x / temp) reaches draws[row] in [0, 1). temp <= 0:
+ * the first maximum. Any top_k; sums are exact to 2^-46 of the largest weight,
+ * and the result does not depend on the launch. probs (optional) receives the
+ * id's probability under the last softmax (1 for temp <= 0). A row without any
+ * value above -inf gives id -1 and probability 0. vocab is at most 2^18. */
+int mf_sample_batch(int* ids, float* probs, const void* logits, int dtype, long long ld, int n_rows, int vocab,
+                    const float* draws, const float* temp, const int* top_k, const float* top_p, const float* min_p,
+                    void* stream);
 
 /* Status bits of the prefill kernels since the last clear (1: a GEMM wait
  * gave up, 2: an attention wait gave up, 4: attention q/k outside the fp16

@@ -30,6 +30,7 @@ MF_STEP_RECORD_BYTES = 32
 MF_STEP_FRAME = 4
 MF_PREFILL_STORE, MF_PREFILL_RESID, MF_PREFILL_SWIGLU = 0, 1, 2
 MF_FRAME_RECORD, MF_FRAME_REPLAY = 0, 1
+MF_ROPE_PLAIN, MF_ROPE_LINEAR, MF_ROPE_NTK, MF_ROPE_YARN = 0, 1, 2, 3
 MF_GEN_STOP_AT_EOS, MF_GEN_MARGINS, MF_GEN_TOKEN_PREFILL = 1, 2, 4
 
 _STATUS = {
@@ -79,8 +80,31 @@ class mf_attn_desc(C.Structure):
                 ("d_head", C.c_int), ("n_split", C.c_int), ("workspace", C.c_void_p), ("kv_dtype", C.c_int)]
 
 
+class mf_paged_kv(C.Structure):
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("page_stride", C.c_longlong),
+                ("head_stride", C.c_longlong), ("row_stride", C.c_longlong), ("page_table", C.c_void_p),
+                ("q_start", C.c_void_p), ("kv_lens", C.c_void_p), ("table_stride", C.c_int), ("max_pages", C.c_int),
+                ("n_pages", C.c_int), ("page_size", C.c_int), ("n_seqs", C.c_int), ("n_kv_heads", C.c_int),
+                ("d_head", C.c_int), ("dtype", C.c_int)]
+
+
+class mf_paged_rope_desc(C.Structure):
+    _fields_ = [("q_out", C.c_void_p), ("q_stride", C.c_longlong), ("qkv", C.c_void_p), ("x_stride", C.c_longlong),
+                ("x_dtype", C.c_int), ("n_tokens", C.c_int), ("n_heads", C.c_int), ("d_rot", C.c_int),
+                ("interleaved", C.c_int), ("mscale", C.c_float), ("eps", C.c_float), ("freqs", C.c_void_p),
+                ("q_norm_w", C.c_void_p), ("k_norm_w", C.c_void_p), ("positions", C.c_void_p)]
+
+
+class mf_paged_attn_desc(C.Structure):
+    _fields_ = [("out", C.c_void_p), ("out_stride", C.c_longlong), ("q", C.c_void_p), ("q_stride", C.c_longlong),
+                ("n_tokens", C.c_int), ("n_heads", C.c_int), ("scale", C.c_float), ("window", C.c_int),
+                ("max_new", C.c_int), ("max_len", C.c_int), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 P = C.c_void_p
 I = C.c_int
+L = C.c_longlong
+D = C.c_double
 U32 = C.c_uint32
 SZ = C.c_size_t
 F = C.c_float
@@ -163,6 +187,11 @@ CUDA_API = {
     "mf_prefill_attention_scratch": (I, [I, I, I, I, P]),
     "mf_prefill_attention_tc": (I, [P, P, P, P, P, I, I, I, I, I, I, P, SZ, I, P]),
     "mf_prefill_status": (I, [P, I]),
+    "mf_rope_freqs": (I, [P, I, D, I, D, D, D, D, P]),
+    "mf_paged_rope_append": (I, [P, P, P]),
+    "mf_paged_attention_workspace_bytes": (SZ, [I, I, I, I, I]),
+    "mf_paged_attention": (I, [P, P, P]),
+    "mf_sample_batch": (I, [P, P, P, I, L, I, I, P, P, P, P, P, P]),
     "mf_topk_workspace_bytes": (SZ, [I, I]),
     "mf_topk": (I, [P, I, I, P, P, P, SZ, P]),
     "mf_sample_step": (I, [P, P, I, F, F, F, P, I, P, P, P, P]),

@@ -1,0 +1,286 @@
+// Entry points of the paged KV cache (include/minfer_cuda.h, "One step of a
+// batch of sequences over a paged KV cache"): argument checks and launches.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdlib>
+#include <mutex>
+
+#include "minfer_cuda.h"
+#include "paged_attn.cuh"
+#include "paged_rope.cuh"
+
+namespace mf {
+int record_error(int code, const char* msg);  // capi.cu: message for mf_last_error
+cudaStream_t resolve_stream(void* stream);    // capi.cu: NULL -> manager stream of the current device
+}  // namespace mf
+
+namespace {
+
+int fail(int code, const char* msg) { return mf::record_error(code, msg); }
+
+bool pdl_on() {
+    const char* e = std::getenv("MF_PDL");
+    return !(e && e[0] == '0');
+}
+
+cudaError_t launch(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t st, void** args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    if (pdl_on()) {
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+    }
+    return cudaLaunchKernelExC(&cfg, fn, args);
+}
+
+int num_sms() {
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) {
+        cudaGetLastError();
+        return 148;
+    }
+    return v;
+}
+
+size_t dtype_bytes(int dtype) { return dtype == MF_F32 ? 4 : 2; }
+bool known_dtype(int dtype) { return dtype == MF_F32 || dtype == MF_F16 || dtype == MF_BF16; }
+bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+// Checks a cache's description and resolves it.
+int resolve_kv(const mf_paged_kv* c, int n_tokens, mf::PagedKv* p) {
+    if (!c || !c->k_pages || !c->v_pages || !c->page_table || !c->q_start || !c->kv_lens)
+        return fail(MF_E_INVALID, "paged cache: null argument");
+    if (!known_dtype(c->dtype)) return fail(MF_E_INVALID, "paged cache: bad dtype");
+    if (c->n_seqs < 0 || n_tokens < 0 || c->n_pages <= 0 || c->max_pages <= 0 || c->n_kv_heads <= 0)
+        return fail(MF_E_INVALID, "paged cache: bad sizes");
+    if (c->table_stride != 0 && c->table_stride < c->max_pages)
+        return fail(MF_E_INVALID, "paged cache: table_stride below max_pages");
+    if (c->d_head != 64 && c->d_head != 128) return fail(MF_E_UNSUPPORTED, "paged cache: d_head must be 64 or 128");
+    if (c->page_size <= 0 || c->page_size % 8 != 0 || c->page_size > (1 << 20))
+        return fail(MF_E_UNSUPPORTED, "paged cache: page_size must be a multiple of 8, up to 2^20");
+    const long long row = c->row_stride ? c->row_stride : c->d_head;
+    const long long head = c->head_stride ? c->head_stride : (long long)c->page_size * c->d_head;
+    const long long page = c->page_stride ? c->page_stride : head * c->n_kv_heads;
+    const long long unit = 16 / (long long)dtype_bytes(c->dtype);
+    if (row < c->d_head || head < c->d_head || page < c->d_head || row % unit || head % unit || page % unit ||
+        !aligned(c->k_pages, 16) || !aligned(c->v_pages, 16))
+        return fail(MF_E_INVALID, "paged cache: pages and strides must be 16-byte aligned, strides at least d_head");
+    if (!aligned(c->page_table, 4) || !aligned(c->q_start, 4) || !aligned(c->kv_lens, 4))
+        return fail(MF_E_INVALID, "paged cache: tables must be 4-byte aligned");
+    p->k = c->k_pages;
+    p->v = c->v_pages;
+    p->page_stride = page;
+    p->head_stride = head;
+    p->row_stride = row;
+    p->table = c->page_table;
+    p->q_start = c->q_start;
+    p->kv_lens = c->kv_lens;
+    p->table_stride = c->table_stride ? c->table_stride : c->max_pages;
+    p->max_pages = c->max_pages;
+    p->n_pages = c->n_pages;
+    p->page_size = c->page_size;
+    p->n_seqs = c->n_seqs;
+    p->n_kv_heads = c->n_kv_heads;
+    p->n_tokens = n_tokens;
+    return MF_OK;
+}
+
+template <typename X, typename T> const void* rope_fn2(int d) {
+    return d == 64 ? (const void*)&mf::paged_rope_kernel<X, T, 64> : (const void*)&mf::paged_rope_kernel<X, T, 128>;
+}
+template <typename X> const void* rope_fn1(int t, int d) {
+    return t == MF_F32   ? rope_fn2<X, float>(d)
+           : t == MF_F16 ? rope_fn2<X, __half>(d)
+                         : rope_fn2<X, __nv_bfloat16>(d);
+}
+const void* rope_fn(int x, int t, int d) {
+    return x == MF_F32 ? rope_fn1<float>(t, d) : x == MF_F16 ? rope_fn1<__half>(t, d) : rope_fn1<__nv_bfloat16>(t, d);
+}
+
+// ---------------------------------------------------------------- attention plans
+struct SimtPlan {
+    const void* kernel;
+    const void* join;
+    size_t smem;
+    int RT;
+};
+template <typename T, int D, int RT> SimtPlan simt_plan3() {
+    SimtPlan s;
+    s.kernel = (const void*)&mf::paged_simt_kernel<T, D, RT>;
+    s.join = (const void*)&mf::paged_join_kernel<T, D, RT, mf::PA_SIMT_KT>;
+    s.smem = mf::paged_simt_smem<RT, D>();
+    s.RT = RT;
+    return s;
+}
+template <typename T> SimtPlan simt_plan1(int d, bool few) {
+    return d == 64 ? (few ? simt_plan3<T, 64, 16>() : simt_plan3<T, 64, 64>())
+                   : (few ? simt_plan3<T, 128, 16>() : simt_plan3<T, 128, 64>());
+}
+SimtPlan simt_plan(int dtype, int d, bool few) {
+    return dtype == MF_F32   ? simt_plan1<float>(d, few)
+           : dtype == MF_F16 ? simt_plan1<__half>(d, few)
+                             : simt_plan1<__nv_bfloat16>(d, few);
+}
+
+// Blocks of `fn` that are resident at once; also sets its shared-memory size.
+int resident(const void* fn, int threads, size_t smem, int* blocks) {
+    static std::mutex mu;
+    std::lock_guard<std::mutex> lk(mu);
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    int per = 0;
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, fn, threads, smem);
+    if (e != cudaSuccess) return fail(MF_E_CUDA, cudaGetErrorString(e));
+    *blocks = std::max(per, 1) * num_sms();
+    return MF_OK;
+}
+
+constexpr int MAX_PER_SM = 4;  // bound of the blocks per SM that the workspace is sized for
+
+size_t part_bytes(int blocks, int RT, int d) { return (size_t)2 * blocks * RT * (d + 2) * sizeof(float); }
+
+}  // namespace
+
+extern "C" {
+
+int mf_rope_freqs(double* out, int d_rot, double base, int scaling, double factor, double orig_ctx, double beta_fast,
+                  double beta_slow, float* mscale) {
+    if (!out || !mscale) return fail(MF_E_INVALID, "null argument");
+    if (d_rot < 2 || d_rot % 2 != 0 || !(base > 1.0) || !std::isfinite(base)) return fail(MF_E_INVALID, "bad d_rot or base");
+    if (scaling < MF_ROPE_PLAIN || scaling > MF_ROPE_YARN) return fail(MF_E_INVALID, "unknown rope scaling");
+    if (scaling != MF_ROPE_PLAIN && !(factor >= 1.0 && std::isfinite(factor))) return fail(MF_E_INVALID, "factor must be at least 1");
+    if (scaling == MF_ROPE_NTK && d_rot < 4) return fail(MF_E_INVALID, "d_rot must be at least 4 with a stretched base");
+    double lo = 0, hi = 1;
+    if (scaling == MF_ROPE_YARN) {
+        if (!(orig_ctx > 0 && beta_fast > beta_slow && beta_slow > 0 && std::isfinite(orig_ctx) && std::isfinite(beta_fast)))
+            return fail(MF_E_INVALID, "need orig_ctx > 0 and beta_fast > beta_slow > 0");
+        // pair index at which a dimension makes `beta` turns over the original context
+        const double two_pi = 6.283185307179586;
+        lo = std::max(std::floor(d_rot * std::log(orig_ctx / (beta_fast * two_pi)) / (2 * std::log(base))), 0.0);
+        hi = std::min(std::ceil(d_rot * std::log(orig_ctx / (beta_slow * two_pi)) / (2 * std::log(base))), d_rot - 1.0);
+        hi = std::max(hi, lo + 1e-3);
+    }
+    if (scaling == MF_ROPE_NTK) base *= std::pow(factor, d_rot / (d_rot - 2.0));
+    for (int j = 0; j < d_rot / 2; ++j) {
+        double f = std::pow(base, -2.0 * j / d_rot);
+        if (scaling == MF_ROPE_LINEAR) f /= factor;
+        if (scaling == MF_ROPE_YARN) {
+            const double ramp = std::min(std::max((j - lo) / (hi - lo), 0.0), 1.0);
+            f = f / factor * ramp + f * (1.0 - ramp);
+        }
+        out[j] = f / 6.283185307179586;
+    }
+    *mscale = scaling == MF_ROPE_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+    return MF_OK;
+}
+
+int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* d, void* stream) {
+    mf::PagedKv p;
+    if (!d) return fail(MF_E_INVALID, "null argument");
+    int rc = resolve_kv(kv, d->n_tokens, &p);
+    if (rc) return rc;
+    if (!d->q_out || !d->qkv || (!d->freqs && d->d_rot > 0)) return fail(MF_E_INVALID, "null argument");
+    if (!known_dtype(d->x_dtype)) return fail(MF_E_INVALID, "bad dtype");
+    if (d->n_heads <= 0 || d->n_heads % kv->n_kv_heads != 0)
+        return fail(MF_E_INVALID, "n_heads must be a positive multiple of n_kv_heads");
+    if (d->d_rot < 0 || d->d_rot > kv->d_head || d->d_rot % 8 != 0)
+        return fail(MF_E_INVALID, "d_rot must be a multiple of 8, at most d_head");
+    if (!(d->eps >= 0.f)) return fail(MF_E_INVALID, "eps must not be negative");
+    const int D = kv->d_head;
+    const long long width = (long long)(d->n_heads + 2 * kv->n_kv_heads) * D;
+    mf::PagedRope r = {};
+    r.q_out = d->q_out;
+    r.q_stride = d->q_stride ? d->q_stride : (long long)d->n_heads * D;
+    r.qkv = d->qkv;
+    r.x_stride = d->x_stride ? d->x_stride : width;
+    const long long ux = 16 / (long long)dtype_bytes(d->x_dtype), uq = 16 / (long long)dtype_bytes(kv->dtype);
+    if (r.q_stride < (long long)d->n_heads * D || r.x_stride < width || r.q_stride % uq || r.x_stride % ux ||
+        !aligned(d->q_out, 16) || !aligned(d->qkv, 16))
+        return fail(MF_E_INVALID, "qkv and q_out: rows must be 16-byte aligned and not overlap");
+    if (!aligned(d->freqs, 8) || !aligned(d->q_norm_w, 4) || !aligned(d->k_norm_w, 4) || !aligned(d->positions, 4))
+        return fail(MF_E_INVALID, "misaligned table");
+    if (d->n_tokens == 0 || kv->n_seqs == 0) return MF_OK;
+    r.freqs = d->freqs;
+    r.q_norm_w = d->q_norm_w;
+    r.k_norm_w = d->k_norm_w;
+    r.positions = d->positions;
+    r.eps = d->eps;
+    r.mscale = d->mscale;
+    r.n_heads = d->n_heads;
+    r.d_rot = d->d_rot;
+    r.interleaved = d->interleaved != 0;
+    // Heads per warp: the angles cost about as much as a few heads, so a warp
+    // takes more heads as soon as the warps still fill the SMs.
+    const int H = d->n_heads + 2 * kv->n_kv_heads;
+    const long long warps = (long long)num_sms() * 32;
+    r.hpw = (int)std::min<long long>(std::max<long long>((long long)d->n_tokens * H / warps, 1), 16);
+    const long long units = (long long)d->n_tokens * ((H + r.hpw - 1) / r.hpw);
+    const long long blocks = (units + mf::ROPE_WARPS - 1) / mf::ROPE_WARPS;
+    if (blocks > 0x7fffffffll) return fail(MF_E_UNSUPPORTED, "too many rows");
+    void* args[] = {&p, &r};
+    cudaError_t e = launch(rope_fn(d->x_dtype, kv->dtype, D), dim3((unsigned)blocks), dim3(mf::ROPE_WARPS * 32), 0,
+                           mf::resolve_stream(stream), args);
+    return e == cudaSuccess ? MF_OK : fail(MF_E_CUDA, cudaGetErrorString(e));
+}
+
+size_t mf_paged_attention_workspace_bytes(int n_tokens, int n_heads, int n_kv_heads, int d_head, int dtype) {
+    if (n_tokens <= 0 || n_heads <= 0 || n_kv_heads <= 0 || (d_head != 64 && d_head != 128) || !known_dtype(dtype)) return 0;
+    return part_bytes(num_sms(), 64, d_head) + part_bytes(MAX_PER_SM * num_sms(), 16, d_head);
+}
+
+int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void* stream) {
+    mf::PagedKv p;
+    if (!d) return fail(MF_E_INVALID, "null argument");
+    int rc = resolve_kv(kv, d->n_tokens, &p);
+    if (rc) return rc;
+    if (!d->out || !d->q) return fail(MF_E_INVALID, "null argument");
+    if (d->n_heads <= 0 || d->n_heads % kv->n_kv_heads != 0)
+        return fail(MF_E_INVALID, "n_heads must be a positive multiple of n_kv_heads");
+    if (d->window < 0 || d->max_new < 0 || d->max_len < 0) return fail(MF_E_INVALID, "window and hints must not be negative");
+    if (!std::isfinite(d->scale)) return fail(MF_E_INVALID, "scale must be finite");
+    const int D = kv->d_head, G = d->n_heads / kv->n_kv_heads;
+    if ((long long)d->n_tokens * G > 0x40000000ll) return fail(MF_E_UNSUPPORTED, "too many query rows");
+    mf::PagedAttn a = {};
+    a.out = d->out;
+    a.q = d->q;
+    a.out_stride = d->out_stride ? d->out_stride : (long long)d->n_heads * D;
+    a.q_stride = d->q_stride ? d->q_stride : (long long)d->n_heads * D;
+    const long long u = 16 / (long long)dtype_bytes(kv->dtype);
+    if (a.out_stride < (long long)d->n_heads * D || a.q_stride < (long long)d->n_heads * D || a.out_stride % u ||
+        a.q_stride % u || !aligned(d->out, 16) || !aligned(d->q, 16))
+        return fail(MF_E_INVALID, "q and out: rows must be 16-byte aligned and not overlap");
+    if (d->n_tokens == 0 || kv->n_seqs == 0) return MF_OK;
+    if (!d->workspace || !aligned(d->workspace, 256) ||
+        d->workspace_bytes < mf_paged_attention_workspace_bytes(d->n_tokens, d->n_heads, kv->n_kv_heads, D, kv->dtype))
+        return fail(MF_E_INVALID, "workspace missing, too small or not 256-byte aligned");
+    a.scale2 = (d->scale == 0.f ? 1.0f / sqrtf((float)D) : d->scale) * 1.4426950408889634f;
+    a.n_heads = d->n_heads;
+    a.G = G;
+    a.window = d->window;
+    a.part = (float*)d->workspace;
+    const int most = std::min(d->max_new > 0 ? d->max_new : d->n_tokens, d->n_tokens);
+    cudaStream_t st = mf::resolve_stream(stream);
+
+    const SimtPlan s = simt_plan(kv->dtype, D, (long long)most * G <= 16);
+    int blocks = 0;
+    rc = resident(s.kernel, mf::PA_SIMT_THREADS, s.smem, &blocks);
+    if (rc) return rc;
+    blocks = std::min(blocks, (s.RT == 64 ? 1 : MAX_PER_SM) * num_sms());
+    void* args[] = {&p, &a};
+    cudaError_t e = launch(s.kernel, dim3(blocks), dim3(mf::PA_SIMT_THREADS), s.smem, st, args);
+    if (e == cudaSuccess && blocks > 1) {
+        void* jargs[] = {&p, &a, &blocks};
+        e = launch(s.join, dim3(blocks - 1), dim3(256), 0, st, jargs);
+    }
+    return e == cudaSuccess ? MF_OK : fail(MF_E_CUDA, cudaGetErrorString(e));
+}
+
+}  // extern "C"

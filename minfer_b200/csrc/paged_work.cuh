@@ -1,0 +1,190 @@
+// How the paged attention kernels for few rows share a batch out.
+//
+// An item is a tile of RT query rows (row r of a sequence = token r / G, head
+// r % G of the group) of one KV head of one sequence; its work is the number
+// of KT-key tiles that its rows see. The items of the whole batch, laid end to
+// end, are cut into equal ranges of tiles, one per CTA, wherever the cut
+// falls: lengths from one key to the longest balance by themselves, and the
+// grid does not depend on them. An item inside one range is finished by its
+// CTA; of one that crosses a cut every CTA leaves (O, m, l) of its part in a
+// slot of its own, and the block of the item's first cut in a second kernel
+// joins them in order (paged_join_kernel). No counters or flags stay behind,
+// and the result does not depend on which CTA ran first.
+#pragma once
+
+#include "paged.cuh"
+
+namespace mf {
+
+struct PagedAttn {
+    void* out;  // [n_tokens][out_stride]
+    long long out_stride;
+    const void* q;  // [n_tokens][q_stride]
+    long long q_stride;
+    float scale2;  // softmax scale * log2(e)
+    int n_heads, G, window;
+    int max_rows;  // sequences of more rows (n_b * G) are another kernel's (0: none are)
+    float* part;   // (O, m, l) of unfinished items: [2 * grid][RT][D], then [2 * grid][RT][2]
+    int* status;   // bit 2: a wait gave up
+    unsigned long long timeout_ns;
+};
+
+// The keys [lo, hi) that rows [r0, r0 + RT) of a sequence see between them.
+struct PagedSpan {
+    int lo, hi;
+};
+MF_DEVICE PagedSpan paged_span(const PagedSeq& s, const PagedAttn& a, int r0, int rows) {
+    const int t0 = r0 / a.G, t1 = (min(r0 + rows, s.n * a.G) - 1) / a.G;
+    PagedSpan k;
+    k.hi = max(s.first + t1 + 1, 0);
+    k.lo = a.window > 0 ? min(max(s.first + t0 - a.window + 1, 0), k.hi) : 0;
+    return k;
+}
+// Number of KT-key tiles of a span; a span without keys still takes one (its rows' zeros are written).
+template <int KT> MF_DEVICE int paged_tiles(const PagedSpan& k) { return max((k.hi + KT - 1) / KT - k.lo / KT, 1); }
+
+// Tiles of one KV head of sequence b (0: no rows, or another kernel's)
+template <int RT, int KT> MF_DEVICE int paged_head_work(const PagedSeq& s, const PagedAttn& a) {
+    const int rows = s.n * a.G;
+    if (rows == 0 || (a.max_rows > 0 && rows > a.max_rows)) return 0;
+    int w = 0;
+    for (int r = 0; r < rows; r += RT) w += paged_tiles<KT>(paged_span(s, a, r, RT));
+    return w;
+}
+
+// A position in the batch's work: item (b, h, r0) that starts at tile `start` of all.
+struct PagedItem {
+    int b, h, r0;
+    long long start;
+    int tiles;
+    PagedSeq s;
+    PagedSpan k;
+};
+
+// Total work, and the item that holds tile `at` (if at < total). Called by the
+// whole block (a multiple of 32 threads, <= 1024); `sh` is shared scratch of 34
+// long longs. Each thread sums a run of sequences; the owner of `at` is found
+// in the block's prefix sums and walked by every thread.
+template <int RT, int KT>
+MF_DEVICE long long paged_find(const PagedKv& p, const PagedAttn& a, long long at_cta, bool as_share, int grid,
+                               long long* sh, long long& share, PagedItem& it) {
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
+    const int run = (p.n_seqs + nt - 1) / nt;
+    const int b0 = min(tid * run, p.n_seqs), b1 = min(b0 + run, p.n_seqs);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += (long long)p.n_kv_heads * paged_head_work<RT, KT>(paged_seq(p, b), a);
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+    }
+    if (lane == 31) sh[warp] = inc;
+    __syncthreads();
+    long long base = 0, total = 0;
+    for (int w = 0; w < (nt >> 5); ++w) {
+        const long long v = sh[w];
+        if (w < warp) base += v;
+        total += v;
+    }
+    share = (total + grid - 1) / grid;
+    const long long at = as_share ? at_cta * share : at_cta;
+    const long long begin = base + inc - mine;
+    __syncthreads();
+    if (mine > 0 && at >= begin && at < begin + mine) {
+        sh[32] = begin;
+        sh[33] = b0;
+    }
+    __syncthreads();
+    it.tiles = 0;
+    if (at >= total) return total;
+    long long w = sh[32];
+    int b = (int)sh[33];
+    for (;; ++b) {
+        const PagedSeq s = paged_seq(p, b);
+        const int hw = paged_head_work<RT, KT>(s, a);
+        if (hw > 0 && at < w + (long long)hw * p.n_kv_heads) {
+            it.b = b;
+            it.s = s;
+            it.h = (int)((at - w) / hw);
+            w += (long long)it.h * hw;
+            break;
+        }
+        w += (long long)hw * p.n_kv_heads;
+    }
+    for (it.r0 = 0;; it.r0 += RT) {
+        it.k = paged_span(it.s, a, it.r0, RT);
+        it.tiles = paged_tiles<KT>(it.k);
+        if (at < w + it.tiles) break;
+        w += it.tiles;
+    }
+    it.start = w;
+    return total;
+}
+
+// The item after `it` (only called while work is left).
+template <int RT, int KT> MF_DEVICE void paged_next(const PagedKv& p, const PagedAttn& a, PagedItem& it) {
+    it.start += it.tiles;
+    it.r0 += RT;
+    if (it.r0 >= it.s.n * a.G) {
+        it.r0 = 0;
+        if (++it.h == p.n_kv_heads) {
+            it.h = 0;
+            do {
+                it.s = paged_seq(p, ++it.b);
+            } while (it.s.n == 0 || (a.max_rows > 0 && it.s.n * a.G > a.max_rows));
+        }
+    }
+    it.k = paged_span(it.s, a, it.r0, RT);
+    it.tiles = paged_tiles<KT>(it.k);
+}
+
+// Joins the parts of every item that a cut divides: block c (1 .. grid - 1)
+// takes the item whose first inner cut is c. Row by row, with m the largest
+// part maximum, out = sum O_i 2^(m_i - m) / sum l_i 2^(m_i - m). A part that
+// saw no key has m = -inf and adds nothing; a row without any key is 0.
+template <typename T, int D, int RT, int KT>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedKv p, const PagedAttn a, int grid) {
+    __shared__ long long sh[34];
+    pdl_launch_dependents();
+    pdl_wait();
+    PagedItem it;
+    long long share;
+    const long long c = (long long)blockIdx.x + 1;
+    const long long total = paged_find<RT, KT>(p, a, c, true, grid, sh, share, it);
+    const long long at = c * share;
+    if (at >= total || it.start == at || it.start / share + 1 != c) return;
+    const int last = (int)((it.start + it.tiles - 1) / share);
+    const int first = (int)c - 1;
+    const int rows = min(RT, it.s.n * a.G - it.r0);
+    const float* ml = a.part + (long long)2 * grid * RT * D;
+    constexpr int V = D / 32;
+    const int lane = threadIdx.x & 31;
+    for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5) {
+        // the first part is its CTA's second slot unless the item begins that CTA's range
+        const int slot0 = 2 * first + (it.start == first * share ? 0 : 1);
+        float m = -INFINITY;
+        for (int i = first; i <= last; ++i) m = fmaxf(m, __ldcg(ml + ((long long)(i == first ? slot0 : 2 * i) * RT + r) * 2));
+        float l = 0.f, o[V] = {};
+        if (m != -INFINITY) {
+            for (int i = first; i <= last; ++i) {
+                const long long at_r = (long long)(i == first ? slot0 : 2 * i) * RT + r;
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(ml) + at_r);
+                const float w = v.x == -INFINITY ? 0.f : exp2f(v.x - m);
+                l = fmaf(v.y, w, l);
+                const PackV<float, V> x = *reinterpret_cast<const PackV<float, V>*>(a.part + at_r * D + lane * V);
+#pragma unroll
+                for (int e = 0; e < V; ++e) o[e] = w > 0.f ? fmaf(x.e[e], w, o[e]) : o[e];
+            }
+        }
+        const float inv = l > 0.f ? 1.0f / l : 0.f;
+        PackV<T, V> y;
+#pragma unroll
+        for (int e = 0; e < V; ++e) y.e[e] = from_f<T>(o[e] * inv);
+        const int row = it.r0 + r;
+        *reinterpret_cast<PackV<T, V>*>(reinterpret_cast<T*>(a.out) + (long long)(it.s.row + row / a.G) * a.out_stride +
+                                        (long long)(it.h * a.G + row % a.G) * D + lane * V) = y;
+    }
+}
+
+}  // namespace mf

@@ -12,7 +12,8 @@ import ctypes as C
 
 import torch
 
-from ._lib import MF_BF16, MF_F16, MF_F32, check, cuda_lib, mf_attn_desc
+from ._lib import (MF_BF16, MF_F16, MF_F32, MF_ROPE_LINEAR, MF_ROPE_NTK, MF_ROPE_PLAIN, MF_ROPE_YARN, check, cuda_lib,
+                   mf_attn_desc, mf_paged_attn_desc, mf_paged_kv, mf_paged_rope_desc)
 
 _lib = cuda_lib()
 
@@ -172,3 +173,152 @@ def lm_head(logits, x, norm_w, eps: float, w, vocab: int, d_model: int, step_sta
             vocab_offset: int = 0, dtype: str | None = None):
     check(_lib.mf_lm_head(_ptr(logits), _ptr(x), _ptr(norm_w), eps, _ptr(w), dtype_code(w, dtype), vocab, d_model,
                           vocab_offset, _ptr(step_state), _ptr(workspace), _stream()))
+
+
+# ---------------------------------------------------------------- a batch of sequences over a paged KV cache
+
+_CODES = {torch.float32: MF_F32, torch.float16: MF_F16, torch.bfloat16: MF_BF16}
+_SCALINGS = {"none": MF_ROPE_PLAIN, "linear": MF_ROPE_LINEAR, "ntk": MF_ROPE_NTK, "yarn": MF_ROPE_YARN}
+
+
+def _tensor(t: torch.Tensor, name: str, dtype, device, dims: int) -> int:
+    """Address of a CUDA tensor on `device` with the given dtype and rank; strides are the caller's business."""
+    if t.dtype is not dtype or t.dim() != dims or t.device != device:
+        raise ValueError(f"{name}: expected a {dims}-d {dtype} tensor on {device}, got {t.dim()}-d {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _vector(t: torch.Tensor | None, name: str, dtype, device, n: int) -> int | None:
+    if t is None:
+        return None
+    p = _tensor(t, name, dtype, device, 1)
+    if t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name}: expected {n} contiguous elements")
+    return p
+
+
+def _rows(t: torch.Tensor, name: str, dtype, device, n: int, width: int) -> tuple[int, int]:
+    """Address and row stride of n rows of `width` contiguous elements: [n, width], or [n, heads, d_head]."""
+    dims = t.dim()
+    p = _tensor(t, name, dtype, device, 3 if dims == 3 else 2)
+    shape, stride = t.shape, t.stride()
+    inner = shape[1] if dims == 2 else shape[1] * shape[2]
+    if shape[0] != n or inner != width or stride[-1] != 1 or (dims == 3 and stride[1] != shape[2]):
+        raise ValueError(f"{name}: expected {n} rows of {width} contiguous elements, got {tuple(shape)} with strides {stride}")
+    return p, stride[0] if n > 1 else width
+
+
+def _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens, device) -> mf_paged_kv:
+    dtype = k_pages.dtype
+    code = _CODES.get(dtype)
+    if code is None or k_pages.dim() != 4 or device.type != "cuda":
+        raise ValueError("k_pages: expected a CUDA tensor [n_pages, n_kv_heads, page_size, d_head] of float32, float16 or bfloat16")
+    kp = k_pages.data_ptr()
+    vp = _tensor(v_pages, "v_pages", dtype, device, 4)
+    n_pages, heads, size, d = shape = k_pages.shape
+    strides = k_pages.stride()
+    if v_pages.shape != shape or v_pages.stride() != strides or strides[3] != 1:
+        raise ValueError("k_pages and v_pages: expected the same shape and strides, heads contiguous")
+    table = _tensor(page_table, "page_table", torch.int32, device, 2)
+    n_seqs, max_pages = page_table.shape
+    if max_pages > 1 and page_table.stride(1) != 1:
+        raise ValueError("page_table: expected contiguous rows")
+    return mf_paged_kv(kp, vp, strides[0], strides[1], strides[2], table,
+                       _vector(q_start, "q_start", torch.int32, device, n_seqs + 1),
+                       _vector(kv_lens, "kv_lens", torch.int32, device, n_seqs),
+                       page_table.stride(0) if n_seqs > 1 else max_pages, max_pages, n_pages, size, n_seqs, heads, d, code)
+
+
+def _on(device, fn, *args) -> None:
+    """fn(*args, stream) on torch's current stream of `device`."""
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, _stream()))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _stream()))
+
+
+def rope_freqs(d_rot: int, base: float, scaling: str = "none", factor: float = 1.0, orig_ctx: float = 0.0,
+               beta_fast: float = 32.0, beta_slow: float = 1.0) -> tuple[torch.Tensor, float]:
+    """Frequencies for paged_rope_append, in turns per position (host tensor, float64 [d_rot / 2]), and the magnitude
+    (mscale). scaling: "none", "linear", "ntk" or "yarn" (which needs orig_ctx)."""
+    if scaling not in _SCALINGS:
+        raise ValueError(f"unknown scaling {scaling!r}")
+    out = torch.empty(max(d_rot, 0) // 2, dtype=torch.float64)
+    mscale = C.c_float()
+    check(_lib.mf_rope_freqs(C.c_void_p(out.data_ptr()), d_rot, base, _SCALINGS[scaling], factor, orig_ctx, beta_fast,
+                             beta_slow, C.byref(mscale)))
+    return out, mscale.value
+
+
+def paged_rope_append(q_out, k_pages, v_pages, page_table, qkv, q_start, kv_lens, freqs, *, interleaved: bool = False,
+                      mscale: float = 1.0, q_norm_w=None, k_norm_w=None, eps: float = 1e-6, positions=None):
+    """Q/K norm (where weights are given), rotary positions and the append to the paged cache, for the new tokens of a
+    batch: rows [q_start[b], q_start[b+1]) of qkv are the last tokens of sequence b, kv_lens[b] long with them.
+
+    k_pages / v_pages: [n_pages, n_kv_heads, page_size, d_head] (any strides with contiguous heads, e.g. a transposed
+    view of [n_pages, page_size, n_kv_heads, d_head]); page_table: int32 [n_seqs, max_pages]; q_out: [n_tokens,
+    n_heads, d_head] in the pages' dtype; qkv: [n_tokens, (n_heads + 2 n_kv_heads) * d_head]; freqs: float64
+    [d_rot / 2] in turns per position (rope_freqs). Rows of no sequence, and the rest of the pages, stay as they are."""
+    device = k_pages.device
+    kv = _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens, device)
+    d, n = kv.d_head, qkv.shape[0]
+    q_width = q_out.shape[1] * (q_out.shape[2] if q_out.dim() == 3 else 1)
+    x_code = _CODES.get(qkv.dtype)
+    if x_code is None:
+        raise ValueError(f"qkv: unsupported dtype {qkv.dtype}")
+    q, q_stride = _rows(q_out, "q_out", k_pages.dtype, device, n, q_width)
+    x, x_stride = _rows(qkv, "qkv", qkv.dtype, device, n, q_width + 2 * kv.n_kv_heads * d)
+    if q_width % d:
+        raise ValueError("q_out: expected whole heads")
+    half = freqs.shape[0]
+    desc = mf_paged_rope_desc(q, q_stride, x, x_stride, x_code, n, q_width // d, 2 * half, interleaved, mscale, eps,
+                              _vector(freqs, "freqs", torch.float64, device, half),
+                              _vector(q_norm_w, "q_norm_w", torch.float32, device, d),
+                              _vector(k_norm_w, "k_norm_w", torch.float32, device, d),
+                              _vector(positions, "positions", torch.int32, device, n))
+    _on(device, _lib.mf_paged_rope_append, C.byref(kv), C.byref(desc))
+
+
+def paged_attention_workspace_bytes(n_tokens: int, n_heads: int, n_kv_heads: int, d_head: int, dtype: torch.dtype) -> int:
+    return int(_lib.mf_paged_attention_workspace_bytes(n_tokens, n_heads, n_kv_heads, d_head, _CODES[dtype]))
+
+
+def paged_attention(out, q, k_pages, v_pages, page_table, q_start, kv_lens, *, scale: float = 0.0, window: int = 0,
+                    max_new: int = 0, max_len: int = 0, workspace=None):
+    """out = attention of the new tokens over the cached positions up to their own (the last `window` of them, 0: all);
+    arguments as in paged_rope_append, out and q [n_tokens, n_heads, d_head]. scale 0 means 1 / sqrt(d_head). max_new
+    and max_len are hints: the most new tokens and the longest length of a sequence. workspace: a uint8 tensor of
+    paged_attention_workspace_bytes, 256-byte aligned, not shared by overlapping calls; None takes one from torch."""
+    device = k_pages.device
+    kv = _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens, device)
+    n, d = q.shape[0], kv.d_head
+    width = q.shape[1] * (q.shape[2] if q.dim() == 3 else 1)
+    qp, q_stride = _rows(q, "q", k_pages.dtype, device, n, width)
+    op, o_stride = _rows(out, "out", k_pages.dtype, device, n, width)
+    if width % d:
+        raise ValueError("q: expected whole heads")
+    if workspace is None:
+        need = _lib.mf_paged_attention_workspace_bytes(n, width // d, kv.n_kv_heads, d, kv.dtype)
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    desc = mf_paged_attn_desc(op, o_stride, qp, q_stride, n, width // d, scale, window, max_new, max_len,
+                              _tensor(workspace, "workspace", torch.uint8, device, 1), workspace.shape[0])
+    _on(device, _lib.mf_paged_attention, C.byref(kv), C.byref(desc))
+
+
+def sample_batch(ids, logits, draws, temp, top_k, top_p, min_p, probs=None):
+    """One id per row of logits [n_rows, vocab] (float32, float16 or bfloat16; rows may be strided): the reference
+    Sampler's filters with row's own temp, top_k, top_p and min_p, and draws[row] in [0, 1) as its random number. ids and
+    top_k are int32, the others float32 vectors of n_rows. probs (optional, float32) receives the ids' probabilities."""
+    device = logits.device
+    code = _CODES.get(logits.dtype)
+    if code is None or logits.dim() != 2 or device.type != "cuda":
+        raise ValueError("logits: expected a 2-d CUDA tensor of float32, float16 or bfloat16")
+    n, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("logits: expected contiguous rows")
+    f = torch.float32
+    _on(device, _lib.mf_sample_batch, _vector(ids, "ids", torch.int32, device, n), _vector(probs, "probs", f, device, n),
+        logits.data_ptr(), code, logits.stride(0) if n > 1 else vocab, n, vocab, _vector(draws, "draws", f, device, n),
+        _vector(temp, "temp", f, device, n), _vector(top_k, "top_k", torch.int32, device, n),
+        _vector(top_p, "top_p", f, device, n), _vector(min_p, "min_p", f, device, n))
