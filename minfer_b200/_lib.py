@@ -191,6 +191,7 @@ CUDA_API = {
     "mf_paged_rope_append": (I, [P, P, P]),
     "mf_paged_attention_workspace_bytes": (SZ, [I, I, I, I, I]),
     "mf_paged_attention": (I, [P, P, P]),
+    "mf_paged_status": (I, [P, I]),
     "mf_sample_batch": (I, [P, P, P, I, L, I, I, P, P, P, P, P, P]),
     "mf_topk_workspace_bytes": (SZ, [I, I]),
     "mf_topk": (I, [P, I, I, P, P, P, SZ, P]),

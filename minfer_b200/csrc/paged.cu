@@ -1,5 +1,6 @@
 // Entry points of the paged KV cache (include/minfer_cuda.h, "One step of a
 // batch of sequences over a paged KV cache"): argument checks and launches.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -9,6 +10,7 @@
 
 #include "minfer_cuda.h"
 #include "paged_attn.cuh"
+#include "paged_fa.cuh"
 #include "paged_rope.cuh"
 
 namespace mf {
@@ -17,6 +19,8 @@ cudaStream_t resolve_stream(void* stream);    // capi.cu: NULL -> manager stream
 }  // namespace mf
 
 namespace {
+
+__device__ int g_paged_status;  // bit 2: a wait of the attention kernels gave up
 
 int fail(int code, const char* msg) { return mf::record_error(code, msg); }
 
@@ -49,6 +53,57 @@ int num_sms() {
         return 148;
     }
     return v;
+}
+
+unsigned long long timeout_ns() {
+    const char* e = std::getenv("MF_PREFILL_TIMEOUT_MS");
+    const long v = (e && *e) ? std::atol(e) : 2000;
+    return 1000000ull * (unsigned long long)(v > 0 ? v : 2000);
+}
+
+int* status_ptr() {
+    static int* p[64] = {nullptr};
+    static std::mutex mu;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!p[dev] && cudaGetSymbolAddress((void**)&p[dev], g_paged_status) != cudaSuccess) return nullptr;
+    return p[dev];
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn tmap_encoder() {
+    static EncodeFn encode = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            encode = (EncodeFn)fn;
+    });
+    return encode;
+}
+
+// Largest power of two that divides page_size, at most `most`: keys of a page that one TMA box can bring in.
+int page_run(int page_size, int most) {
+    int r = page_size & -page_size;
+    return std::min(r, most);
+}
+
+// Map of 16-bit pages: (d, row of the page, head, page), boxes of 64 elements x `run` rows, 128-byte swizzle.
+int page_tmap(CUtensorMap* tm, const void* base, const mf::PagedKv& p, int D, int dtype, int run) {
+    EncodeFn encode = tmap_encoder();
+    if (!encode) return fail(MF_E_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)p.page_size, (cuuint64_t)p.n_kv_heads, (cuuint64_t)p.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)p.row_stride * 2, (cuuint64_t)p.head_stride * 2, (cuuint64_t)p.page_stride * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)run, 1, 1}, es[4] = {1, 1, 1, 1};
+    const CUresult r = encode(tm, dtype == MF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                              const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? MF_OK : fail(MF_E_INVALID, "the pages' strides do not fit a tensor map");
 }
 
 size_t dtype_bytes(int dtype) { return dtype == MF_F32 ? 4 : 2; }
@@ -145,6 +200,25 @@ int resident(const void* fn, int threads, size_t smem, int* blocks) {
 
 constexpr int MAX_PER_SM = 4;  // bound of the blocks per SM that the workspace is sized for
 
+// Shares of the keys in which the chunk kernel works when its row tiles alone
+// leave SMs idle (1: none).
+int chunk_split(int n_tokens, int n_heads, int n_kv_heads) {
+    const long long ctas = ((long long)n_tokens * (n_heads / n_kv_heads) + mf::PF_ROWS - 1) / mf::PF_ROWS * n_kv_heads;
+    return (int)std::min<long long>(std::max<long long>(num_sms() / ctas, 1), 16);
+}
+
+template <typename T, int D> const void* fa_fn2(bool join) {
+    return join ? (const void*)&mf::paged_fa_join_kernel<T, D> : (const void*)&mf::paged_fa_kernel<T, D>;
+}
+const void* fa_fn(int dtype, int d, bool join) {
+    return dtype == MF_F16 ? (d == 64 ? fa_fn2<__half, 64>(join) : fa_fn2<__half, 128>(join))
+                           : (d == 64 ? fa_fn2<__nv_bfloat16, 64>(join) : fa_fn2<__nv_bfloat16, 128>(join));
+}
+
+// Sequences of more query rows (new tokens x heads of a group) than this go to
+// the chunk kernel, which works on 256 rows at a time.
+constexpr int FEW_ROWS = 32;
+
 size_t part_bytes(int blocks, int RT, int d) { return (size_t)2 * blocks * RT * (d + 2) * sizeof(float); }
 
 }  // namespace
@@ -233,7 +307,9 @@ int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* d, voi
 
 size_t mf_paged_attention_workspace_bytes(int n_tokens, int n_heads, int n_kv_heads, int d_head, int dtype) {
     if (n_tokens <= 0 || n_heads <= 0 || n_kv_heads <= 0 || (d_head != 64 && d_head != 128) || !known_dtype(dtype)) return 0;
-    return part_bytes(num_sms(), 64, d_head) + part_bytes(MAX_PER_SM * num_sms(), 16, d_head);
+    const size_t few = std::max(part_bytes(num_sms(), 64, d_head), part_bytes(MAX_PER_SM * num_sms(), 16, d_head));
+    const size_t split = (size_t)chunk_split(n_tokens, n_heads, n_kv_heads) * n_tokens * n_heads * (d_head + 2) * sizeof(float);
+    return few + (dtype == MF_F32 ? 0 : split);
 }
 
 int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void* stream) {
@@ -269,17 +345,68 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
     const int most = std::min(d->max_new > 0 ? d->max_new : d->n_tokens, d->n_tokens);
     cudaStream_t st = mf::resolve_stream(stream);
 
-    const SimtPlan s = simt_plan(kv->dtype, D, (long long)most * G <= 16);
-    int blocks = 0;
-    rc = resident(s.kernel, mf::PA_SIMT_THREADS, s.smem, &blocks);
-    if (rc) return rc;
-    blocks = std::min(blocks, (s.RT == 64 ? 1 : MAX_PER_SM) * num_sms());
-    void* args[] = {&p, &a};
-    cudaError_t e = launch(s.kernel, dim3(blocks), dim3(mf::PA_SIMT_THREADS), s.smem, st, args);
-    if (e == cudaSuccess && blocks > 1) {
-        void* jargs[] = {&p, &a, &blocks};
-        e = launch(s.join, dim3(blocks - 1), dim3(256), 0, st, jargs);
+    a.status = status_ptr();
+    if (!a.status) return fail(MF_E_CUDA, "status symbol");
+    a.timeout_ns = timeout_ns();
+
+    // 16-bit pages: sequences of more than FEW_ROWS rows go to the tensor-core
+    // chunk kernel. A batch of one sequence is served by one kernel alone.
+    const bool chunks = kv->dtype != MF_F32 && (long long)most * G > FEW_ROWS;
+    const bool few = !chunks || kv->n_seqs > 1;
+    cudaError_t e = cudaSuccess;
+    if (chunks) {
+        mf::PagedFa f = {};
+        f.run = page_run(p.page_size, mf::PF_KT);
+        f.min_rows = few ? FEW_ROWS : 0;
+        a.max_rows = few ? FEW_ROWS : 0;
+        f.n_split = chunk_split(d->n_tokens, d->n_heads, kv->n_kv_heads);
+        if (d->max_len > 0) f.n_split = std::min(f.n_split, std::max(1, d->max_len / (4 * mf::PF_KT)));
+        const size_t rows = (size_t)d->n_tokens * d->n_heads;
+        f.part_o = a.part + (mf_paged_attention_workspace_bytes(d->n_tokens, d->n_heads, kv->n_kv_heads, D, MF_F32) + 3) / 4;
+        f.part_ml = (float2*)(f.part_o + f.n_split * rows * D);
+        CUtensorMap tk, tv;
+        rc = page_tmap(&tk, p.k, p, D, kv->dtype, f.run);
+        if (!rc) rc = page_tmap(&tv, p.v, p, D, kv->dtype, f.run);
+        if (rc) return rc;
+        const void* fn = fa_fn(kv->dtype, D, false);
+        const size_t smem = D == 64 ? mf::pf_smem<64>() : mf::pf_smem<128>();
+        int unused = 0;
+        rc = resident(fn, mf::PF_THREADS, smem, &unused);
+        if (rc) return rc;
+        // every tile of every such sequence: at most T G / 256 whole ones, and one more for each sequence
+        const long long tg = (long long)d->n_tokens * G;
+        const long long tiles = tg / mf::PF_ROWS + std::min<long long>(kv->n_seqs, tg / (f.min_rows + 1));
+        if (tiles * kv->n_kv_heads > 0x7fffffffll) return fail(MF_E_UNSUPPORTED, "too many query rows");
+        void* args[] = {&tk, &tv, &p, &a, &f};
+        e = launch(fn, dim3((unsigned)(tiles * kv->n_kv_heads), (unsigned)f.n_split), dim3(mf::PF_THREADS), smem, st, args);
+        if (e == cudaSuccess && f.n_split > 1) {
+            void* jargs[] = {&p, &a, &f};
+            e = launch(fa_fn(kv->dtype, D, true), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, jargs);
+        }
     }
+    if (few && e == cudaSuccess) {
+        const SimtPlan s = simt_plan(kv->dtype, D, chunks || (long long)most * G <= 16);
+        int blocks = 0;
+        rc = resident(s.kernel, mf::PA_SIMT_THREADS, s.smem, &blocks);
+        if (rc) return rc;
+        blocks = std::min(blocks, (s.RT == 64 ? 1 : MAX_PER_SM) * num_sms());
+        void* args[] = {&p, &a};
+        e = launch(s.kernel, dim3(blocks), dim3(mf::PA_SIMT_THREADS), s.smem, st, args);
+        if (e == cudaSuccess && blocks > 1) {
+            void* jargs[] = {&p, &a, &blocks};
+            e = launch(s.join, dim3(blocks - 1), dim3(256), 0, st, jargs);
+        }
+    }
+    return e == cudaSuccess ? MF_OK : fail(MF_E_CUDA, cudaGetErrorString(e));
+}
+
+int mf_paged_status(int* status, int clear) {
+    if (!status) return fail(MF_E_INVALID, "null argument");
+    int* p = status_ptr();
+    if (!p) return fail(MF_E_CUDA, "status symbol");
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpy(status, p, sizeof(int), cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess && clear) e = cudaMemset(p, 0, sizeof(int));
     return e == cudaSuccess ? MF_OK : fail(MF_E_CUDA, cudaGetErrorString(e));
 }
 

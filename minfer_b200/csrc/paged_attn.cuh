@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
         auto store = [&](int r, int c, float4 v) {
             if (r >= rows) return;
             if (whole) {
-                const float inv = l_s[r] > 0.f ? 1.0f / l_s[r] : 0.f;
+                const float inv = l_s[r] == 0.f ? 0.f : 1.0f / l_s[r];
                 const int row = it.r0 + r;
                 PackV<T, 4> y;
                 y.e[0] = from_f<T>(v.x * inv);

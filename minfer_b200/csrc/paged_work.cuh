@@ -174,10 +174,10 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedKv p, const 
                 l = fmaf(v.y, w, l);
                 const PackV<float, V> x = *reinterpret_cast<const PackV<float, V>*>(a.part + at_r * D + lane * V);
 #pragma unroll
-                for (int e = 0; e < V; ++e) o[e] = w > 0.f ? fmaf(x.e[e], w, o[e]) : o[e];
+                for (int e = 0; e < V; ++e) o[e] = w != 0.f ? fmaf(x.e[e], w, o[e]) : o[e];
             }
         }
-        const float inv = l > 0.f ? 1.0f / l : 0.f;
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
         PackV<T, V> y;
 #pragma unroll
         for (int e = 0; e < V; ++e) y.e[e] = from_f<T>(o[e] * inv);

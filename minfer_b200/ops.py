@@ -306,6 +306,13 @@ def paged_attention(out, q, k_pages, v_pages, page_table, q_start, kv_lens, *, s
     _on(device, _lib.mf_paged_attention, C.byref(kv), C.byref(desc))
 
 
+def paged_status(clear: bool = True) -> int:
+    """Status bits of paged_attention's kernels on the current device since the last clear (2: a wait gave up)."""
+    status = C.c_int()
+    check(_lib.mf_paged_status(C.byref(status), int(clear)))
+    return status.value
+
+
 def sample_batch(ids, logits, draws, temp, top_k, top_p, min_p, probs=None):
     """One id per row of logits [n_rows, vocab] (float32, float16 or bfloat16; rows may be strided): the reference
     Sampler's filters with row's own temp, top_k, top_p and min_p, and draws[row] in [0, 1) as its random number. ids and
