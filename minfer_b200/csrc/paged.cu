@@ -11,6 +11,7 @@
 #include "minfer_cuda.h"
 #include "paged_attn.cuh"
 #include "paged_fa.cuh"
+#include "paged_few.cuh"
 #include "paged_rope.cuh"
 
 namespace mf {
@@ -162,28 +163,29 @@ const void* rope_fn(int x, int t, int d) {
 }
 
 // ---------------------------------------------------------------- attention plans
-struct SimtPlan {
+// A kernel for few rows and the one that joins its parts.
+struct FewPlan {
     const void* kernel;
     const void* join;
     size_t smem;
-    int RT;
+    int threads, RT;
 };
-template <typename T, int D, int RT> SimtPlan simt_plan3() {
-    SimtPlan s;
-    s.kernel = (const void*)&mf::paged_simt_kernel<T, D, RT>;
-    s.join = (const void*)&mf::paged_join_kernel<T, D, RT, mf::PA_SIMT_KT>;
-    s.smem = mf::paged_simt_smem<RT, D>();
-    s.RT = RT;
-    return s;
+template <int D, int RT> FewPlan simt_plan() {
+    return {(const void*)&mf::paged_simt_kernel<float, D, RT>, (const void*)&mf::paged_join_kernel<float, D, RT, mf::PA_SIMT_KT>,
+            (size_t)mf::paged_simt_smem<RT, D>(), mf::PA_SIMT_THREADS, RT};
 }
-template <typename T> SimtPlan simt_plan1(int d, bool few) {
-    return d == 64 ? (few ? simt_plan3<T, 64, 16>() : simt_plan3<T, 64, 64>())
-                   : (few ? simt_plan3<T, 128, 16>() : simt_plan3<T, 128, 64>());
+template <typename T, int D, int MT> FewPlan mma_plan() {
+    return {(const void*)&mf::paged_few_kernel<T, D, MT>, (const void*)&mf::paged_join_kernel<T, D, 16 * MT, mf::PW_KT>,
+            (size_t)mf::pw_smem<D, MT>(), mf::PW_THREADS, 16 * MT};
 }
-SimtPlan simt_plan(int dtype, int d, bool few) {
-    return dtype == MF_F32   ? simt_plan1<float>(d, few)
-           : dtype == MF_F16 ? simt_plan1<__half>(d, few)
-                             : simt_plan1<__nv_bfloat16>(d, few);
+template <typename T> FewPlan mma_plan2(int d, bool one) {
+    return d == 64 ? (one ? mma_plan<T, 64, 1>() : mma_plan<T, 64, 2>()) : (one ? mma_plan<T, 128, 1>() : mma_plan<T, 128, 2>());
+}
+// `rows`: the most rows of a sequence, as far as known
+FewPlan few_plan(int dtype, int d, long long rows) {
+    const bool one = rows <= 16;
+    if (dtype == MF_F32) return d == 64 ? (one ? simt_plan<64, 16>() : simt_plan<64, 64>()) : (one ? simt_plan<128, 16>() : simt_plan<128, 64>());
+    return dtype == MF_F16 ? mma_plan2<__half>(d, one) : mma_plan2<__nv_bfloat16>(d, one);
 }
 
 // Blocks of `fn` that are resident at once; also sets its shared-memory size.
@@ -198,7 +200,8 @@ int resident(const void* fn, int threads, size_t smem, int* blocks) {
     return MF_OK;
 }
 
-constexpr int MAX_PER_SM = 4;  // bound of the blocks per SM that the workspace is sized for
+// Blocks per SM that the workspace of the kernels for few rows is sized for.
+int per_sm(int RT) { return RT == 16 ? 4 : RT == 32 ? 2 : 1; }
 
 // Shares of the keys in which the chunk kernel works when its row tiles alone
 // leave SMs idle (1: none).
@@ -307,7 +310,7 @@ int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* d, voi
 
 size_t mf_paged_attention_workspace_bytes(int n_tokens, int n_heads, int n_kv_heads, int d_head, int dtype) {
     if (n_tokens <= 0 || n_heads <= 0 || n_kv_heads <= 0 || (d_head != 64 && d_head != 128) || !known_dtype(dtype)) return 0;
-    const size_t few = std::max(part_bytes(num_sms(), 64, d_head), part_bytes(MAX_PER_SM * num_sms(), 16, d_head));
+    const size_t few = part_bytes(num_sms(), 64, d_head);  // the same for 2 blocks per SM of 32 rows and 4 of 16
     const size_t split = (size_t)chunk_split(n_tokens, n_heads, n_kv_heads) * n_tokens * n_heads * (d_head + 2) * sizeof(float);
     return few + (dtype == MF_F32 ? 0 : split);
 }
@@ -385,13 +388,23 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
         }
     }
     if (few && e == cudaSuccess) {
-        const SimtPlan s = simt_plan(kv->dtype, D, chunks || (long long)most * G <= 16);
+        const FewPlan s = few_plan(kv->dtype, D, chunks ? std::min<long long>(FEW_ROWS, (long long)most * G) : (long long)most * G);
         int blocks = 0;
-        rc = resident(s.kernel, mf::PA_SIMT_THREADS, s.smem, &blocks);
+        rc = resident(s.kernel, s.threads, s.smem, &blocks);
         if (rc) return rc;
-        blocks = std::min(blocks, (s.RT == 64 ? 1 : MAX_PER_SM) * num_sms());
-        void* args[] = {&p, &a};
-        e = launch(s.kernel, dim3(blocks), dim3(mf::PA_SIMT_THREADS), s.smem, st, args);
+        blocks = std::min(blocks, per_sm(s.RT) * num_sms());
+        if (kv->dtype == MF_F32) {
+            void* args[] = {&p, &a};
+            e = launch(s.kernel, dim3(blocks), dim3(s.threads), s.smem, st, args);
+        } else {
+            int run = page_run(p.page_size, mf::PW_KT);
+            CUtensorMap tk, tv;
+            rc = page_tmap(&tk, p.k, p, D, kv->dtype, run);
+            if (!rc) rc = page_tmap(&tv, p.v, p, D, kv->dtype, run);
+            if (rc) return rc;
+            void* args[] = {&tk, &tv, &p, &a, &run};
+            e = launch(s.kernel, dim3(blocks), dim3(s.threads), s.smem, st, args);
+        }
         if (e == cudaSuccess && blocks > 1) {
             void* jargs[] = {&p, &a, &blocks};
             e = launch(s.join, dim3(blocks - 1), dim3(256), 0, st, jargs);
