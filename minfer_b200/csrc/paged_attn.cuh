@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
     const T* vb = reinterpret_cast<const T*>(p.v);
 
     for (long long w = w0; w < w1;) {
-        const int j0 = (int)(w - it.start), j1 = (int)min((long long)it.tiles, w1 - it.start);
+        const int j0 = (int)max(w - it.start, 0ll), j1 = (int)min((long long)it.tiles, w1 - it.start);
+        if (j1 <= 0) break;  // only the item's first unit is in this range
         const int rows = min(RT, it.s.n * a.G - it.r0);
         const int kt0 = it.k.lo / KT;
         __syncthreads();
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
         }
         __syncthreads();
         const bool whole = j0 == 0 && j1 == it.tiles;
-        const long long slot = 2ll * blockIdx.x + (w == w0 ? 0 : 1);
+        const long long slot = 2ll * blockIdx.x + (j0 > 0 ? 0 : 1);
         float* part = a.part + slot * RT * D;
         float* ml = a.part + 2ll * gridDim.x * RT * D + slot * RT * 2;
         auto store = [&](int r, int c, float4 v) {

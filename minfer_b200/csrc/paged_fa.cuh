@@ -209,10 +209,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                     rest &= rest - 1;
                     const int pg = __shfl_sync(0xffffffffu, page, i), k0 = __shfl_sync(0xffffffffu, c0, i);
                     const T* src = reinterpret_cast<const T*>(p.v) + (pg < 0 ? 0 : pg * p.page_stride + (long long)h * p.head_stride + (long long)(k0 % p.page_size) * p.row_stride);
+#pragma unroll 8
                     for (int e = lane; e < R * (D / 8); e += 32) {
                         const int r = e / (D / 8), c = e % (D / 8), key = k0 + r;
                         uint4 v = make_uint4(0, 0, 0, 0);
-                        if (pg >= 0 && key >= span.lo && key < span.hi) v = *reinterpret_cast<const uint4*>(src + r * p.row_stride + c * 8);
+                        if (pg >= 0 && key >= span.lo && key < span.hi) v = __ldg(reinterpret_cast<const uint4*>(src + r * p.row_stride + c * 8));
                         const int row = i * R + r;
                         *reinterpret_cast<uint4*>(dst + (c >> 3) * PF_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
                     }

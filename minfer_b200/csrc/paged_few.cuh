@@ -12,8 +12,8 @@
 // tensor pipe is far from its limit, and a 16-row tile of tcgen05 does not
 // exist). They meet only at the end of an item, to join the four parts through
 // shared memory. As in the chunk kernel the maximum moves only when it grows
-// by more than 2^8, and runs that no row sees are not read (scores masked, V
-// rows zeroed).
+// by more than 2^8; runs that no row sees are not read, and of a run that is
+// seen in part the other rows are masked (scores) and zeroed (V, in registers).
 #pragma once
 
 #include "paged_fa.cuh"
@@ -92,47 +92,32 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
         const int R = run, nr = PW_KT / R;
         int n = 0;  // tiles issued
         for (long long w = w0; w < w1 && !failed;) {
-            const int j0 = (int)(w - it.start), j1 = (int)min((long long)it.tiles, w1 - it.start);
+            const int j0 = (int)max(w - it.start, 0ll), j1 = (int)min((long long)it.tiles, w1 - it.start);
+            if (j1 <= 0) break;  // only the item's first unit is in this range
             const int k_first = it.k.lo / PW_KT * PW_KT;
             for (int j = j0; j < j1; ++j, ++n) {
                 const int st = n % ST;
                 const int c0 = k_first + j * PW_KT + lane * R;  // this lane's run: keys [c0, c0 + R)
                 const int page = lane < nr && c0 < it.k.hi && c0 + R > it.k.lo ? paged_page(p, it.b, c0) : -1;
                 const int off = c0 % p.page_size;
-                const bool seen_whole = c0 >= it.k.lo && c0 + R <= it.k.hi;
-                const unsigned kbox = __ballot_sync(0xffffffffu, page >= 0);
-                const unsigned vbox = __ballot_sync(0xffffffffu, page >= 0 && seen_whole);
-                unsigned rest = ((1u << nr) - 1u) & ~vbox;
+                const unsigned boxes = __ballot_sync(0xffffffffu, page >= 0);
                 if (n >= ST) mbar_wait(&free_[st], ((uint32_t)(n / ST) & 1u) ^ 1u, deadline, failed);
                 failed = __any_sync(0xffffffffu, failed);
                 if (failed) break;
                 uint8_t* kd = smem + st * 2 * TILE;
                 uint8_t* vd = kd + TILE;
-                while (rest) {  // V rows that no row sees are zeros; a run seen in part is copied row by row
-                    const int i = __ffs(rest) - 1;
-                    rest &= rest - 1;
-                    const int pg = __shfl_sync(0xffffffffu, page, i), k0 = __shfl_sync(0xffffffffu, c0, i), o = __shfl_sync(0xffffffffu, off, i);
-                    const T* src = reinterpret_cast<const T*>(p.v) + (pg < 0 ? 0 : pg * p.page_stride + (long long)it.h * p.head_stride + (long long)o * p.row_stride);
-                    for (int e = lane; e < R * (D / 8); e += 32) {
-                        const int r = e / (D / 8), c = e % (D / 8), key = k0 + r, row = i * R + r;
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (pg >= 0 && key >= it.k.lo && key < it.k.hi) v = *reinterpret_cast<const uint4*>(src + r * p.row_stride + c * 8);
-                        *reinterpret_cast<uint4*>(vd + (c >> 3) * HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
-                    }
-                }
-                __syncwarp();
                 if (lane == 0) {
                     uint32_t ok = 0;  // per 8 keys
-                    for (int i = 0; i < PW_KT / 8; ++i) ok |= (kbox >> (8 * i / R) & 1u) << i;
+                    for (int i = 0; i < PW_KT / 8; ++i) ok |= (boxes >> (8 * i / R) & 1u) << i;
                     pages_s[st] = ok;
-                    mbar_expect_tx(&full[st], (uint32_t)(__popc(kbox) + __popc(vbox)) * R * D * 2);
+                    mbar_expect_tx(&full[st], (uint32_t)__popc(boxes) * R * D * 4);
                 }
                 __syncwarp();
                 if (page >= 0) {
 #pragma unroll
                     for (int x = 0; x < D / 64; ++x) {
                         tma_load_4d(kd + x * HALF + lane * R * 128, &tk, &full[st], 64 * x, off, it.h, page);
-                        if (seen_whole) tma_load_4d(vd + x * HALF + lane * R * 128, &tv, &full[st], 64 * x, off, it.h, page);
+                        tma_load_4d(vd + x * HALF + lane * R * 128, &tv, &full[st], 64 * x, off, it.h, page);
                     }
                 }
             }
@@ -150,7 +135,8 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
         const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;  // a negative scale goes into Q's sign
         int n = 0;
         for (long long w = w0; w < w1;) {
-            const int j0 = (int)(w - it.start), j1 = (int)min((long long)it.tiles, w1 - it.start);
+            const int j0 = (int)max(w - it.start, 0ll), j1 = (int)min((long long)it.tiles, w1 - it.start);
+            if (j1 <= 0) break;  // only the item's first unit is in this range
             const int rows = min(RT, it.s.n * a.G - it.r0);
             const int k_first = it.k.lo / PW_KT * PW_KT;
             const T* qb = reinterpret_cast<const T*>(a.q) + (long long)it.s.row * a.q_stride + (long long)it.h * a.G * D;
@@ -287,6 +273,19 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                     pa[mt][2] = pf_pack<T>(s[mt][1][0], s[mt][1][1]);
                     pa[mt][3] = pf_pack<T>(s[mt][1][2], s[mt][1][3]);
                 }
+                // V rows that no row of the item sees are zeros, whatever the tile holds there (element pairs of
+                // two neighbouring keys each, keys 2 (lane % 4) and 8 on)
+                uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+                const bool cut = k0 < it.k.lo || k0 + 16 > it.k.hi || ok != 3u;
+                if (cut) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const int key = k0 + 8 * t + (lane & 3) * 2;
+                        keep[t] = !(ok >> t & 1u) ? 0u
+                                                  : (key >= it.k.lo && key < it.k.hi ? 0xffffu : 0u) |
+                                                        (key + 1 >= it.k.lo && key + 1 < it.k.hi ? 0xffff0000u : 0u);
+                    }
+                }
                 {
                     const int key = kw + (((lane >> 3) & 1) << 3) + (lane & 7);
                     const uint32_t row = vd + key * 128;
@@ -295,6 +294,12 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                         const int c = 2 * d + (lane >> 4);
                         uint32_t b[4];
                         ldsm4t(b, row + (c >> 3) * HALF + (((c & 7) ^ (key & 7)) << 4));
+                        if (cut) {
+                            b[0] &= keep[0];
+                            b[1] &= keep[1];
+                            b[2] &= keep[0];
+                            b[3] &= keep[1];
+                        }
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
                             mma16<T>(o[mt][2 * d], pa[mt], b[0], b[1]);
@@ -316,7 +321,7 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                     if ((lane & 3) == 0) ml_s[warp * RT + 16 * mt + 8 * e + (lane >> 2)] = make_float2(m[mt][e], l[mt][e]);
                 }
             const bool whole = j0 == 0 && j1 == it.tiles;
-            const long long slot = 2ll * blockIdx.x + (w == w0 ? 0 : 1);
+            const long long slot = 2ll * blockIdx.x + (j0 > 0 ? 0 : 1);
             float* part = a.part + slot * RT * D;
             float* part_ml = a.part + 2ll * gridDim.x * RT * D + slot * RT * 2;
 #pragma unroll

@@ -2,14 +2,17 @@
 //
 // An item is a tile of RT query rows (row r of a sequence = token r / G, head
 // r % G of the group) of one KV head of one sequence; its work is the number
-// of KT-key tiles that its rows see. The items of the whole batch, laid end to
-// end, are cut into equal ranges of tiles, one per CTA, wherever the cut
-// falls: lengths from one key to the longest balance by themselves, and the
-// grid does not depend on them. An item inside one range is finished by its
-// CTA; of one that crosses a cut every CTA leaves (O, m, l) of its part in a
-// slot of its own, and the block of the item's first cut in a second kernel
-// joins them in order (paged_join_kernel). No counters or flags stay behind,
-// and the result does not depend on which CTA ran first.
+// of KT-key tiles that its rows see, after one unit for its beginning and end
+// (queries, join, output: about a tile's time; without it a CTA of 55 one-tile
+// items ran four times as long as one of a few long items). The items of the
+// whole batch, laid end to end, are cut into equal ranges, one per CTA,
+// wherever the cut falls: lengths from one key to the longest balance by
+// themselves, and the grid does not depend on them. An item whose tiles lie
+// inside one range is finished by its CTA; of one whose tiles a cut divides
+// every CTA leaves (O, m, l) of its part in a slot of its own, and the block
+// of the item's first inner cut in a second kernel joins them in order
+// (paged_join_kernel). No counters or flags stay behind, and the result does
+// not depend on which CTA ran first.
 #pragma once
 
 #include "paged.cuh"
@@ -24,7 +27,7 @@ struct PagedAttn {
     float scale2;  // softmax scale * log2(e)
     int n_heads, G, window;
     int max_rows;  // sequences of more rows (n_b * G) are another kernel's (0: none are)
-    float* part;   // (O, m, l) of unfinished items: [2 * grid][RT][D], then [2 * grid][RT][2]
+    float* part;   // (O, m, l) of divided items: [2 * grid][RT][D], then [2 * grid][RT][2]
     int* status;   // bit 2: a wait gave up
     unsigned long long timeout_ns;
 };
@@ -48,11 +51,11 @@ template <int RT, int KT> MF_DEVICE int paged_head_work(const PagedSeq& s, const
     const int rows = s.n * a.G;
     if (rows == 0 || (a.max_rows > 0 && rows > a.max_rows)) return 0;
     int w = 0;
-    for (int r = 0; r < rows; r += RT) w += paged_tiles<KT>(paged_span(s, a, r, RT));
+    for (int r = 0; r < rows; r += RT) w += 1 + paged_tiles<KT>(paged_span(s, a, r, RT));
     return w;
 }
 
-// A position in the batch's work: item (b, h, r0) that starts at tile `start` of all.
+// Item (b, h, r0) of the batch: its tiles are the units [start, start + tiles) of all, after the one at start - 1.
 struct PagedItem {
     int b, h, r0;
     long long start;
@@ -61,7 +64,7 @@ struct PagedItem {
     PagedSpan k;
 };
 
-// Total work, and the item that holds tile `at` (if at < total). Called by the
+// Total work, and the item that holds unit `at` (if at < total). Called by the
 // whole block (a multiple of 32 threads, <= 1024); `sh` is shared scratch of 34
 // long longs. Each thread sums a run of sequences; the owner of `at` is found
 // in the block's prefix sums and walked by every thread.
@@ -115,16 +118,16 @@ MF_DEVICE long long paged_find(const PagedKv& p, const PagedAttn& a, long long a
     for (it.r0 = 0;; it.r0 += RT) {
         it.k = paged_span(it.s, a, it.r0, RT);
         it.tiles = paged_tiles<KT>(it.k);
-        if (at < w + it.tiles) break;
-        w += it.tiles;
+        if (at < w + 1 + it.tiles) break;
+        w += 1 + it.tiles;
     }
-    it.start = w;
+    it.start = w + 1;
     return total;
 }
 
 // The item after `it` (only called while work is left).
 template <int RT, int KT> MF_DEVICE void paged_next(const PagedKv& p, const PagedAttn& a, PagedItem& it) {
-    it.start += it.tiles;
+    it.start += it.tiles + 1;
     it.r0 += RT;
     if (it.r0 >= it.s.n * a.G) {
         it.r0 = 0;
@@ -153,7 +156,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedKv p, const 
     const long long c = (long long)blockIdx.x + 1;
     const long long total = paged_find<RT, KT>(p, a, c, true, grid, sh, share, it);
     const long long at = c * share;
-    if (at >= total || it.start == at || it.start / share + 1 != c) return;
+    if (at >= total || at <= it.start || it.start / share + 1 != c) return;
     const int last = (int)((it.start + it.tiles - 1) / share);
     const int first = (int)c - 1;
     const int rows = min(RT, it.s.n * a.G - it.r0);
@@ -161,8 +164,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedKv p, const 
     constexpr int V = D / 32;
     const int lane = threadIdx.x & 31;
     for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5) {
-        // the first part is its CTA's second slot unless the item begins that CTA's range
-        const int slot0 = 2 * first + (it.start == first * share ? 0 : 1);
+        // a CTA's slot 0 is for the item that its range begins inside of, slot 1 for the one it ends inside of
+        const int slot0 = 2 * first + 1;
         float m = -INFINITY;
         for (int i = first; i <= last; ++i) m = fmaxf(m, __ldcg(ml + ((long long)(i == first ? slot0 : 2 * i) * RT + r) * 2));
         float l = 0.f, o[V] = {};
