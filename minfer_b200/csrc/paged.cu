@@ -175,7 +175,7 @@ template <int D, int RT> FewPlan simt_plan() {
             (size_t)mf::paged_simt_smem<RT, D>(), mf::PA_SIMT_THREADS, RT};
 }
 template <typename T, int D, int MT> FewPlan mma_plan() {
-    return {(const void*)&mf::paged_few_kernel<T, D, MT>, (const void*)&mf::paged_join_kernel<T, D, 16 * MT, mf::PW_KT>,
+    return {(const void*)&mf::paged_few_kernel<T, D, MT>, (const void*)&mf::paged_join_kernel<T, D, 16 * MT, mf::pw_kt<D>()>,
             (size_t)mf::pw_smem<D, MT>(), mf::PW_THREADS, 16 * MT};
 }
 template <typename T> FewPlan mma_plan2(int d, bool one) {
@@ -397,7 +397,7 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
             void* args[] = {&p, &a};
             e = launch(s.kernel, dim3(blocks), dim3(s.threads), s.smem, st, args);
         } else {
-            int run = page_run(p.page_size, mf::PW_KT);
+            int run = page_run(p.page_size, D == 64 ? mf::pw_kt<64>() : mf::pw_kt<128>());
             CUtensorMap tk, tv;
             rc = page_tmap(&tk, p.k, p, D, kv->dtype, run);
             if (!rc) rc = page_tmap(&tv, p.v, p, D, kv->dtype, run);

@@ -3,11 +3,12 @@
 // positions (pos - window, pos].
 //
 // Bound by memory: each K and V row is read once per KV head and meets the
-// RT <= 32 query rows of its group. A CTA takes a range of the batch's 64-key
-// tiles (paged_work.cuh), so that lengths need not match. One warp keeps a
-// ring of tiles in flight (two CTAs per SM, about 190 KB of copies
-// outstanding), one TMA box per run of R keys of a page; four warps take 16
-// keys of every tile each, with their own running maximum, sum and O
+// RT <= 32 query rows of its group. A CTA takes a range of the batch's key
+// tiles of 32 KB (paged_work.cuh), so that lengths need not match. One warp
+// keeps a ring of tiles in flight (two CTAs per SM, about 190 KB of copies
+// outstanding), one TMA box per run of R keys of a page; four warps take a
+// quarter of the keys of every tile each (64-wide heads: 32 keys, since with
+// 16 a warp's fixed cost per tile outweighed its copies), with their own running maximum, sum and O
 // (mma.sync m16n8k16, rows padded to 16: at two flops per byte and row the
 // tensor pipe is far from its limit, and a 16-row tile of tcgen05 does not
 // exist). They meet only at the end of an item, to join the four parts through
@@ -20,15 +21,15 @@
 
 namespace mf {
 
-constexpr int PW_KT = 64;
+template <int D> constexpr int pw_kt() { return D == 128 ? 64 : 128; }  // keys per tile: 32 KB of K and V either way
 constexpr int PW_WARPS = 4;                       // consumers
 constexpr int PW_THREADS = (PW_WARPS + 1) * 32;   // and the producer
 constexpr int PW_COLS = 32;                       // columns of O joined at a time
 constexpr int PW_LD = PW_COLS + 8;
-template <int D, int MT> constexpr int pw_stages() { return (D == 128 ? 6 : 12) / (MT == 1 ? 2 : 3); }  // two CTAs fit an SM
-template <int D> constexpr int pw_tile() { return PW_KT * D * 2; }
+template <int MT> constexpr int pw_stages() { return MT == 1 ? 3 : 2; }  // two CTAs fit an SM
+template <int D> constexpr int pw_tile() { return pw_kt<D>() * D * 2; }
 template <int D, int MT> constexpr int pw_smem() {
-    return pw_stages<D, MT>() * 2 * pw_tile<D>() + PW_WARPS * 16 * MT * (PW_LD + 2) * 4 + (MT > 1 ? 16 * MT * D * 2 : 0) + 1024;
+    return pw_stages<MT>() * 2 * pw_tile<D>() + PW_WARPS * 16 * MT * (PW_LD + 2) * 4 + (MT > 1 ? 16 * MT * D * 2 : 0) + 1024;
 }
 
 MF_DEVICE void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -60,7 +61,8 @@ template <typename T, int D, int MT>
 __global__ void __launch_bounds__(PW_THREADS, 2)
     paged_few_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const PagedKv p,
                      const PagedAttn a, const int run) {
-    constexpr int RT = 16 * MT, ST = pw_stages<D, MT>(), TILE = pw_tile<D>(), HALF = PW_KT * 128;
+    constexpr int RT = 16 * MT, ST = pw_stages<MT>(), KT = pw_kt<D>(), TILE = pw_tile<D>(), HALF = KT * 128;
+    constexpr int KW = KT / PW_WARPS;  // keys of one warp: 16 or 32
     extern __shared__ uint8_t pw_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pw_smem_raw) + 1023) & ~(uintptr_t)1023);
     float* join = reinterpret_cast<float*>(smem + ST * 2 * TILE);  // [warp][RT][PW_LD]
@@ -82,22 +84,22 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
     pdl_wait();
     PagedItem it;
     long long share;
-    const long long total = paged_find<RT, PW_KT>(p, a, blockIdx.x, true, gridDim.x, sh, share, it);
+    const long long total = paged_find<RT, KT>(p, a, blockIdx.x, true, gridDim.x, sh, share, it);
     const long long w0 = blockIdx.x * share, w1 = min(w0 + share, total);
     if (w0 >= w1) return;
     const unsigned long long deadline = globaltimer_ns() + a.timeout_ns;
     bool failed = false;
 
     if (warp == PW_WARPS) {
-        const int R = run, nr = PW_KT / R;
+        const int R = run, nr = KT / R;
         int n = 0;  // tiles issued
         for (long long w = w0; w < w1 && !failed;) {
             const int j0 = (int)max(w - it.start, 0ll), j1 = (int)min((long long)it.tiles, w1 - it.start);
             if (j1 <= 0) break;  // only the item's first unit is in this range
-            const int k_first = it.k.lo / PW_KT * PW_KT;
+            const int k_first = it.k.lo / KT * KT;
             for (int j = j0; j < j1; ++j, ++n) {
                 const int st = n % ST;
-                const int c0 = k_first + j * PW_KT + lane * R;  // this lane's run: keys [c0, c0 + R)
+                const int c0 = k_first + j * KT + lane * R;  // this lane's run: keys [c0, c0 + R)
                 const int page = lane < nr && c0 < it.k.hi && c0 + R > it.k.lo ? paged_page(p, it.b, c0) : -1;
                 const int off = c0 % p.page_size;
                 const unsigned boxes = __ballot_sync(0xffffffffu, page >= 0);
@@ -108,7 +110,7 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                 uint8_t* vd = kd + TILE;
                 if (lane == 0) {
                     uint32_t ok = 0;  // per 8 keys
-                    for (int i = 0; i < PW_KT / 8; ++i) ok |= (boxes >> (8 * i / R) & 1u) << i;
+                    for (int i = 0; i < KT / 8; ++i) ok |= (boxes >> (8 * i / R) & 1u) << i;
                     pages_s[st] = ok;
                     mbar_expect_tx(&full[st], (uint32_t)__popc(boxes) * R * D * 4);
                 }
@@ -122,7 +124,7 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                 }
             }
             w = it.start + j1;
-            if (w < w1 && !failed) paged_next<RT, PW_KT>(p, a, it);
+            if (w < w1 && !failed) paged_next<RT, KT>(p, a, it);
         }
         if (failed) {
             // let the copies in flight land before shared memory goes away
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
             const int j0 = (int)max(w - it.start, 0ll), j1 = (int)min((long long)it.tiles, w1 - it.start);
             if (j1 <= 0) break;  // only the item's first unit is in this range
             const int rows = min(RT, it.s.n * a.G - it.r0);
-            const int k_first = it.k.lo / PW_KT * PW_KT;
+            const int k_first = it.k.lo / KT * KT;
             const T* qb = reinterpret_cast<const T*>(a.q) + (long long)it.s.row * a.q_stride + (long long)it.h * a.G * D;
             auto q_row = [&](int r) { return qb + (long long)((it.r0 + r) / a.G) * a.q_stride + (long long)((it.r0 + r) % a.G) * D; };
             uint32_t qf[MT == 1 ? D / 16 : 1][4];
@@ -191,55 +193,59 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                 const int st = n % ST;
                 mbar_wait(&full[st], (uint32_t)(n / ST) & 1u, deadline, failed);
                 const uint32_t kd = smem_u32(smem + st * 2 * TILE), vd = kd + TILE;
-                const int kw = 16 * warp, k0 = k_first + j * PW_KT + kw;  // this warp's 16 keys
-                float s[MT][2][4];
+                const int kw = KW * warp, k0 = k_first + j * KT + kw;  // this warp's keys
+                float s[MT][KW / 8][4];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[mt][0][e] = s[mt][1][e] = 0.f;
-                {
-                    const int key = kw + ((lane >> 4) << 3) + (lane & 7);
-                    const uint32_t row = kd + key * 128;
+                    for (int t = 0; t < KW / 8; ++t) s[mt][t][0] = s[mt][t][1] = s[mt][t][2] = s[mt][t][3] = 0.f;
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const int c = 2 * k + ((lane >> 3) & 1);
+                for (int k = 0; k < D / 16; ++k) {
+                    uint32_t qa[MT][4];
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        if constexpr (MT == 1) {
+                            qa[0][0] = qf[k][0], qa[0][1] = qf[k][1], qa[0][2] = qf[k][2], qa[0][3] = qf[k][3];
+                        } else {
+                            const int r = 16 * mt + (lane & 15), cq = 2 * k + (lane >> 4);
+                            ldsm4(qa[mt], smem_u32(q_s) + r * (D * 2) + ((cq ^ (r & 7)) << 4));
+                        }
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < KW / 16; ++kk) {
+                        const int key = kw + 16 * kk + ((lane >> 4) << 3) + (lane & 7), c = 2 * k + ((lane >> 3) & 1);
                         uint32_t b[4];
-                        ldsm4(b, row + (c >> 3) * HALF + (((c & 7) ^ (key & 7)) << 4));
+                        ldsm4(b, kd + key * 128 + (c >> 3) * HALF + (((c & 7) ^ (key & 7)) << 4));
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
-                            if constexpr (MT == 1) {
-                                mma16<T>(s[mt][0], qf[k], b[0], b[1]);
-                                mma16<T>(s[mt][1], qf[k], b[2], b[3]);
-                            } else {
-                                uint32_t qa[4];
-                                const int r = 16 * mt + (lane & 15), cq = 2 * k + (lane >> 4);
-                                ldsm4(qa, smem_u32(q_s) + r * (D * 2) + ((cq ^ (r & 7)) << 4));
-                                mma16<T>(s[mt][0], qa, b[0], b[1]);
-                                mma16<T>(s[mt][1], qa, b[2], b[3]);
-                            }
+                            mma16<T>(s[mt][2 * kk], qa[mt], b[0], b[1]);
+                            mma16<T>(s[mt][2 * kk + 1], qa[mt], b[2], b[3]);
                         }
                     }
                 }
-                const uint32_t ok = pages_s[st] >> (2 * warp) & 3u;
-                if (!(k0 + 15 <= hi_all && k0 >= lo_all && ok == 3u)) {
+                constexpr uint32_t ALL = (1u << (KW / 8)) - 1;
+                const uint32_t ok = pages_s[st] >> (KW / 8 * warp) & ALL;
+                if (!(k0 + KW - 1 <= hi_all && k0 >= lo_all && ok == ALL)) {
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int t = 0; t < 2; ++t)
+                        for (int t = 0; t < KW / 8; ++t)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const int key = k0 + 8 * t + (lane & 3) * 2 + (e & 1);
                                 if (!(ok >> t & 1u) || key > pos[mt][e >> 1] || key < lo[mt][e >> 1]) s[mt][t][e] = -INFINITY;
                             }
                 }
-                uint32_t pa[MT][4];
+                uint32_t pa[MT][KW / 16][4];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     float alpha[2];
                     bool bump = false;
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float mx = fmaxf(fmaxf(s[mt][0][2 * e], s[mt][0][2 * e + 1]), fmaxf(s[mt][1][2 * e], s[mt][1][2 * e + 1]));
+                        float mx = fmaxf(s[mt][0][2 * e], s[mt][0][2 * e + 1]);
+#pragma unroll
+                        for (int t = 1; t < KW / 8; ++t) mx = fmaxf(mx, fmaxf(s[mt][t][2 * e], s[mt][t][2 * e + 1]));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * c2;
                         const bool up = mx > m[mt][e] + 8.f;
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                         m[mt][e] = mu;
                         float sum = 0.f;
 #pragma unroll
-                        for (int t = 0; t < 2; ++t)
+                        for (int t = 0; t < KW / 8; ++t)
 #pragma unroll
                             for (int u = 0; u < 2; ++u) {
                                 const float x = ex2_approx(fmaf(s[mt][t][2 * e + u], c2, -base));
@@ -268,42 +274,45 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                             o[mt][d][3] *= alpha[1];
                         }
                     }
-                    pa[mt][0] = pf_pack<T>(s[mt][0][0], s[mt][0][1]);
-                    pa[mt][1] = pf_pack<T>(s[mt][0][2], s[mt][0][3]);
-                    pa[mt][2] = pf_pack<T>(s[mt][1][0], s[mt][1][1]);
-                    pa[mt][3] = pf_pack<T>(s[mt][1][2], s[mt][1][3]);
+#pragma unroll
+                    for (int kk = 0; kk < KW / 16; ++kk) {
+                        pa[mt][kk][0] = pf_pack<T>(s[mt][2 * kk][0], s[mt][2 * kk][1]);
+                        pa[mt][kk][1] = pf_pack<T>(s[mt][2 * kk][2], s[mt][2 * kk][3]);
+                        pa[mt][kk][2] = pf_pack<T>(s[mt][2 * kk + 1][0], s[mt][2 * kk + 1][1]);
+                        pa[mt][kk][3] = pf_pack<T>(s[mt][2 * kk + 1][2], s[mt][2 * kk + 1][3]);
+                    }
                 }
-                // V rows that no row of the item sees are zeros, whatever the tile holds there (element pairs of
-                // two neighbouring keys each, keys 2 (lane % 4) and 8 on)
-                uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-                const bool cut = k0 < it.k.lo || k0 + 16 > it.k.hi || ok != 3u;
+                // V rows that no row of the item sees are zeros, whatever the tile holds there (a register holds
+                // the rows of two neighbouring keys, 2 (lane % 4) and the next, of a run of 8)
+                uint32_t keep[KW / 8];
+                const bool cut = k0 < it.k.lo || k0 + KW > it.k.hi || ok != ALL;
                 if (cut) {
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
+                    for (int t = 0; t < KW / 8; ++t) {
                         const int key = k0 + 8 * t + (lane & 3) * 2;
                         keep[t] = !(ok >> t & 1u) ? 0u
                                                   : (key >= it.k.lo && key < it.k.hi ? 0xffffu : 0u) |
                                                         (key + 1 >= it.k.lo && key + 1 < it.k.hi ? 0xffff0000u : 0u);
                     }
                 }
-                {
-                    const int key = kw + (((lane >> 3) & 1) << 3) + (lane & 7);
-                    const uint32_t row = vd + key * 128;
+#pragma unroll
+                for (int kk = 0; kk < KW / 16; ++kk) {
+                    const int key = kw + 16 * kk + (((lane >> 3) & 1) << 3) + (lane & 7);
 #pragma unroll
                     for (int d = 0; d < D / 16; ++d) {
                         const int c = 2 * d + (lane >> 4);
                         uint32_t b[4];
-                        ldsm4t(b, row + (c >> 3) * HALF + (((c & 7) ^ (key & 7)) << 4));
+                        ldsm4t(b, vd + key * 128 + (c >> 3) * HALF + (((c & 7) ^ (key & 7)) << 4));
                         if (cut) {
-                            b[0] &= keep[0];
-                            b[1] &= keep[1];
-                            b[2] &= keep[0];
-                            b[3] &= keep[1];
+                            b[0] &= keep[2 * kk];
+                            b[1] &= keep[2 * kk + 1];
+                            b[2] &= keep[2 * kk];
+                            b[3] &= keep[2 * kk + 1];
                         }
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
-                            mma16<T>(o[mt][2 * d], pa[mt], b[0], b[1]);
-                            mma16<T>(o[mt][2 * d + 1], pa[mt], b[2], b[3]);
+                            mma16<T>(o[mt][2 * d], pa[mt][kk], b[0], b[1]);
+                            mma16<T>(o[mt][2 * d + 1], pa[mt][kk], b[2], b[3]);
                         }
                     }
                 }
@@ -368,7 +377,7 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                 named_bar_sync(1, PW_WARPS * 32);
             }
             w = it.start + j1;
-            if (w < w1) paged_next<RT, PW_KT>(p, a, it);
+            if (w < w1) paged_next<RT, KT>(p, a, it);
         }
     }
     if (failed) atomicOr(a.status, 2);
