@@ -33,6 +33,7 @@ namespace mf {
 constexpr int SB_THREADS = 512;
 constexpr int SB_BINS = 512;        // one per thread
 constexpr int SB_LIST = 64;         // candidates left to one warp (two per lane)
+constexpr int SB_SORT = 2048;       // candidates that one block sorts
 constexpr int SB_MAX_CLUSTER = 8;
 constexpr int SB_MAX_VOCAB = 1 << 18;  // 2^18 weights of at most 2^45: sums below 2^63
 constexpr double SB_ONE = 35184372088832.0;  // 2^45
@@ -89,15 +90,23 @@ struct SbBorder {
 };
 
 struct SbShared {
-    uint32_t cnt[SB_BINS];
-    uint32_t part[3][SB_BINS];  // weights in three parts of 16 bits: 32-bit shared atomics, no overflow below 2^16 terms
-    u64 wsum[SB_BINS];          // their sum, what the other blocks read
+    union {
+        struct {
+            uint32_t cnt[SB_BINS];
+            uint32_t part[3][SB_BINS];  // weights in three parts of 16 bits: 32-bit shared atomics, no overflow below 2^16 terms
+            u64 wsum[SB_BINS];          // their sum, what the other blocks read
+        };
+        u64 sorted[SB_SORT];  // candidates of the whole row (its first block)
+    };
+    u64 cand[SB_SORT];          // (key, ~index) of the block's candidates
     u64 best;                   // (key, ~index) of the block's largest
     u64 scan[34];
+    uint32_t scan_c[32];
     u64 found[4];
     uint32_t list_n;
     uint32_t list_key[SB_LIST], list_idx[SB_LIST];
     uint32_t ties;
+    uint32_t first;             // smallest position asked for
 };
 
 struct SbRow {
@@ -109,6 +118,15 @@ struct SbRow {
 };
 
 enum SbMode { SB_COUNT, SB_WEIGHT };
+
+// Where a border falls among the level-1 bins of the whole row.
+struct SbLevel {
+    int bin;
+    u64 before;     // running sum up to the bin
+    u64 total;      // over the prefix
+    uint32_t in_bin, upto;  // candidates in the bin, and up to its end
+    double target;
+};
 
 // exp((x - top) / T) in multiples of 2^-45
 MF_DEVICE u64 sb_weight(float x, float top, double inv_t) {
@@ -139,6 +157,40 @@ MF_DEVICE u64 sb_scan(u64 v, SbShared* sh, u64& total) {
     return v + base;
 }
 
+// Inclusive scans of a u64 and a count per thread.
+MF_DEVICE u64 sb_scan2(u64 v, uint32_t& c, SbShared* sh, u64& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 u = __shfl_up_sync(0xffffffffu, v, o);
+        const uint32_t d = __shfl_up_sync(0xffffffffu, c, o);
+        if (lane >= o) {
+            v += u;
+            c += d;
+        }
+    }
+    __syncthreads();
+    if (lane == 31) {
+        sh->scan[warp] = v;
+        sh->scan_c[warp] = c;
+    }
+    __syncthreads();
+    u64 base = 0;
+    uint32_t base_c = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < SB_THREADS / 32; ++w) {
+        const u64 x = sh->scan[w];
+        if (w < warp) {
+            base += x;
+            base_c += sh->scan_c[w];
+        }
+        total += x;
+    }
+    c += base_c;
+    return v + base;
+}
+
 // Smallest key of level-1 bin `bin` or below it in the order (monotone search).
 MF_DEVICE uint32_t sb_bin_low(float top, int bin) {
     uint32_t lo = sb_key(-INFINITY), hi = sb_key(top);  // bin(hi) = 0 <= bin
@@ -148,6 +200,146 @@ MF_DEVICE uint32_t sb_bin_low(float top, int bin) {
         else lo = mid + 1;
     }
     return lo;
+}
+
+// Adds one candidate to a bin.
+template <int MODE> MF_DEVICE void sb_add(SbShared* sh, int bin, float x, float top, double inv_t) {
+    if (MODE == SB_WEIGHT) {
+        const u64 w = sb_weight(x, top, inv_t);
+        if (w) {
+            atomicAdd(&sh->part[0][bin], (uint32_t)(w & 0xffff));
+            atomicAdd(&sh->part[1][bin], (uint32_t)((w >> 16) & 0xffff));
+            atomicAdd(&sh->part[2][bin], (uint32_t)(w >> 32));
+        }
+    }
+    atomicAdd(&sh->cnt[bin], 1u);
+}
+
+// The bin in which the running sum over the prefix `in` reaches the target:
+// `want` ones, or share * (the sum) for weights. The block's bins must be zero
+// and in step (sb_clear). The same in every block of the cluster.
+MF_DEVICE void sb_clear(SbShared* sh) {
+    const int tid = threadIdx.x;
+    sh->cnt[tid] = 0;
+    sh->part[0][tid] = sh->part[1][tid] = sh->part[2][tid] = 0;
+    if (tid == 0) sh->first = ~0u;
+}
+template <int MODE>
+MF_DEVICE SbLevel sb_level(const SbRow& r, const SbBorder& in, double inv_t, u64 want, double share) {
+    SbShared* sh = r.sh;
+    const int tid = threadIdx.x;
+    const uint32_t whole = in.key == 0 ? 1 : 0;  // the prefix is everything
+    for (int i = tid; i < r.n; i += SB_THREADS) {
+        const uint32_t k = r.keys[i];
+        if (!whole && !in.keeps(k, r.base + i)) continue;
+        const float x = sb_value(k);
+        sb_add<MODE>(sh, sb_bin(r.top, x), x, r.top, inv_t);
+    }
+    __syncthreads();
+    if (MODE == SB_WEIGHT)
+        sh->wsum[tid] = (u64)sh->part[0][tid] + ((u64)sh->part[1][tid] << 16) + ((u64)sh->part[2][tid] << 32);
+    cluster_sync_all();
+    uint32_t c = 0;
+    u64 w = 0;
+    for (int q = 0; q < r.size; ++q) {
+        c += sb_ld32(&sh->cnt[tid], q);
+        if (MODE == SB_WEIGHT) w += sb_ld64(&sh->wsum[tid], q);
+    }
+    if (MODE == SB_COUNT) w = c;
+    SbLevel v;
+    uint32_t upto = c;
+    const u64 inc = sb_scan2(w, upto, sh, v.total);
+    v.target = MODE == SB_COUNT ? (double)want : share * (double)v.total;
+    const bool hit = c > 0 && (double)inc >= v.target;
+    const unsigned hits = __ballot_sync(0xffffffffu, hit);
+    if ((tid & 31) == 0 && hits) atomicMin(&sh->first, (uint32_t)tid + __ffs(hits) - 1);
+    __syncthreads();
+    v.bin = sh->first;
+    if (tid == v.bin) {
+        sh->found[1] = inc - w;
+        sh->found[2] = (u64)upto << 32 | c;
+    }
+    cluster_sync_all();  // every block has read these bins
+    v.before = sh->found[1];
+    v.in_bin = (uint32_t)sh->found[2];
+    v.upto = (uint32_t)(sh->found[2] >> 32);
+    return v;
+}
+
+// Brings the candidates with keys in [lo, hi] of the prefix `in` to the row's
+// first block and sorts them there (value, then index): n <= SB_SORT of them
+// in all. False in the other blocks, which have nothing more to do.
+MF_DEVICE bool sb_gather(const SbRow& r, const SbBorder& in, uint32_t lo, uint32_t hi, int n) {
+    SbShared* sh = r.sh;
+    const int tid = threadIdx.x;
+    if (tid == 0) sh->list_n = 0;
+    __syncthreads();
+    for (int i = tid; i < r.n; i += SB_THREADS) {
+        const uint32_t k = r.keys[i];
+        if (k < lo || k > hi || !in.keeps(k, r.base + i)) continue;
+        sh->cand[atomicAdd(&sh->list_n, 1u)] = (u64)k << 32 | (uint32_t)~(r.base + i);
+    }
+    cluster_sync_all();
+    if (r.rank == 0) {
+        int m = 32;
+        while (m < n) m *= 2;
+        int at = 0;
+        for (int q = 0; q < r.size; ++q) {
+            const int nq = sb_ld32(&sh->list_n, q);
+            for (int i = tid; i < nq; i += SB_THREADS) sh->sorted[at + i] = sb_ld64(&sh->cand[i], q);
+            at += nq;
+        }
+        for (int i = n + tid; i < m; i += SB_THREADS) sh->sorted[i] = 0;
+        __syncthreads();
+        for (int size = 2; size <= m; size *= 2)
+            for (int stride = size / 2; stride > 0; stride /= 2) {
+                for (int i = tid; i < m / 2; i += SB_THREADS) {
+                    const int x = 2 * i - (i & (stride - 1)), y = x + stride;
+                    const u64 u = sh->sorted[x], v = sh->sorted[y];
+                    if ((u < v) == ((x & size) == 0)) {
+                        sh->sorted[x] = v;
+                        sh->sorted[y] = u;
+                    }
+                }
+                __syncthreads();
+            }
+    }
+    cluster_sync_all();  // the lists have been read
+    return r.rank == 0;
+}
+
+// Position of the first of the n sorted candidates at which before + (running
+// sum of weights) reaches share * total, or target if share < 0; n - 1 if none
+// does. total 0: the sum over the n. Sets `sum` to that total.
+MF_DEVICE int sb_first(const SbRow& r, int n, double inv_t, u64 before, u64 total, double share, u64& sum) {
+    SbShared* sh = r.sh;
+    const int tid = threadIdx.x;
+    constexpr int E = SB_SORT / SB_THREADS;
+    u64 w[E], mine = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int i = tid * E + e;
+        w[e] = i < n ? sb_weight(sb_value((uint32_t)(sh->sorted[i] >> 32)), r.top, inv_t) : 0;
+        mine += w[e];
+    }
+    u64 all;
+    u64 run = before + sb_scan(mine, sh, all) - mine;
+    sum = total ? total : all;
+    const double target = share * (double)sum;
+    if (tid == 0) sh->first = n - 1;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        run += w[e];
+        if (tid * E + e < n && (double)run >= target) {
+            atomicMin(&sh->first, (uint32_t)(tid * E + e));
+            break;
+        }
+    }
+    __syncthreads();
+    const int at = sh->first;
+    __syncthreads();
+    return at;
 }
 
 // First candidate of the prefix `in` at which the running sum reaches the
@@ -386,6 +578,7 @@ __global__ void __launch_bounds__(SB_THREADS) sample_batch_kernel(const SampleBa
     }
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     if (tid == 0) sh.best = 0;
+    sb_clear(&sh);
     __syncthreads();
     if (lane == 0) atomicMax(&sh.best, best);
     cluster_sync_all();
@@ -403,12 +596,12 @@ __global__ void __launch_bounds__(SB_THREADS) sample_batch_kernel(const SampleBa
     const bool none = top_key == sb_key(-INFINITY);  // nothing to choose from
     double prob = 1.0;
     if (!none && temp > 0.f) {
-        SbBorder kept = {0u, ~0u};  // everything
-        u64 sum;
-        if (top_k > 0 && top_k < a.vocab) kept = sb_find<SB_COUNT>(r, kept, 1.0, (u64)top_k, -1.0, sum);
-        if (top_p < 1.f) kept = sb_find<SB_WEIGHT>(r, kept, 1.0, 0, (double)fmaxf(top_p, 0.f), sum);
+        const SbBorder all = {0u, ~0u};
+        const bool cut_k = top_k > 0 && top_k < a.vocab, cut_p = top_p < 1.f;
+        const double share_p = (double)fmaxf(top_p, 0.f), inv_t = 1.0 / (double)temp;
+        const double draw = (double)fminf(fmaxf(a.draws[row], 0.f), 0.99999994f);
+        SbBorder likely = all;  // the smallest value at least min_p as likely as the first: x >= top + log(min_p)
         if (min_p > 0.f) {
-            // the smallest value at least min_p as likely as the first: x >= top + log(min_p)
             const double thr = min_p < 1.f ? (double)r.top + log((double)min_p) : (double)r.top;
             uint32_t lo = sb_key(-INFINITY), hi = top_key;
             while (lo < hi) {
@@ -416,12 +609,51 @@ __global__ void __launch_bounds__(SB_THREADS) sample_batch_kernel(const SampleBa
                 if ((double)sb_value(mid) >= thr) hi = mid;
                 else lo = mid + 1;
             }
-            const SbBorder m = {lo, ~0u};
-            if (m.before(kept)) kept = m;
+            likely.key = lo;
         }
-        const double inv_t = 1.0 / (double)temp;
-        const double draw = (double)fminf(fmaxf(a.draws[row], 0.f), 0.99999994f);
-        pick = sb_find<SB_WEIGHT>(r, kept, inv_t, 0, draw, sum);
+        u64 sum = 0;
+        bool done = false;
+        if (cut_k || cut_p) {
+            const SbLevel v = cut_k ? sb_level<SB_COUNT>(r, all, 1.0, (u64)top_k, -1.0) : sb_level<SB_WEIGHT>(r, all, 1.0, 0, share_p);
+            if (v.upto <= SB_SORT) {
+                // the candidates down to the bin of the first border: what is kept is among the first of them
+                if (!sb_gather(r, all, sb_bin_low(r.top, v.bin), top_key, (int)v.upto)) return;
+                int n = cut_k ? top_k : (int)v.upto;
+                if (cut_p) n = sb_first(r, n, 1.0, 0, cut_k ? 0 : v.total, share_p, sum) + 1;
+                if (min_p > 0.f) {
+                    if (tid == 0) sh.first = n;
+                    __syncthreads();
+                    for (int i = tid; i < n; i += SB_THREADS)
+                        if ((uint32_t)(sh.sorted[i] >> 32) < likely.key) atomicMin(&sh.first, (uint32_t)i);
+                    __syncthreads();
+                    n = sh.first;
+                    __syncthreads();
+                }
+                const u64 got = sh.sorted[sb_first(r, n, inv_t, 0, 0, draw, sum)];
+                pick.key = (uint32_t)(got >> 32);
+                pick.idx = ~(uint32_t)got;
+                done = true;
+            }
+        } else {
+            const SbLevel v = sb_level<SB_WEIGHT>(r, likely, inv_t, 0, draw);
+            if (v.in_bin <= SB_SORT) {
+                // the candidates of the draw's bin
+                const uint32_t lo = sb_bin_low(r.top, v.bin), hi = v.bin > 0 ? sb_bin_low(r.top, v.bin - 1) - 1 : top_key;
+                if (!sb_gather(r, likely, lo, hi, (int)v.in_bin)) return;
+                const u64 got = sh.sorted[sb_first(r, (int)v.in_bin, inv_t, v.before, v.total, draw, sum)];
+                pick.key = (uint32_t)(got >> 32);
+                pick.idx = ~(uint32_t)got;
+                done = true;
+            }
+        }
+        if (!done) {
+            // many candidates down to the border: filter by filter, by descent
+            SbBorder kept = all;
+            if (cut_k) kept = sb_find<SB_COUNT>(r, kept, 1.0, (u64)top_k, -1.0, sum);
+            if (cut_p) kept = sb_find<SB_WEIGHT>(r, kept, 1.0, 0, share_p, sum);
+            if (likely.before(kept)) kept = likely;
+            pick = sb_find<SB_WEIGHT>(r, kept, inv_t, 0, draw, sum);
+        }
         const float v = sb_value(pick.key);
         const double e = v == r.top ? 1.0 : exp(((double)v - (double)r.top) * inv_t);
         prob = e * SB_ONE / (double)sum;
