@@ -12,8 +12,7 @@
 // target.
 //
 // A row lives in the shared memory of one thread-block cluster: the logits are
-// read from memory once, as order-preserving 32-bit keys, and every later pass
-// runs on chip. A border is found by descent: 512 bins of 1/16 below the top,
+// read from memory once, and every later pass runs on chip. A border is found by descent: 512 bins of 1/16 below the top,
 // the bin that holds the border cut into 512 ranges of keys, and so on, until
 // a few candidates are left, which one warp orders, or one value, whose ties
 // are counted out by index. Per level the bins of the cluster's blocks are
@@ -33,7 +32,7 @@ namespace mf {
 constexpr int SB_THREADS = 512;
 constexpr int SB_BINS = 512;        // one per thread
 constexpr int SB_LIST = 64;         // candidates left to one warp (two per lane)
-constexpr int SB_SORT = 2048;       // candidates that one block sorts
+constexpr int SB_FEW = 2048;        // candidates that one block orders: four per thread
 constexpr int SB_MAX_CLUSTER = 8;
 constexpr int SB_MAX_VOCAB = 1 << 18;  // 2^18 weights of at most 2^45: sums below 2^63
 constexpr double SB_ONE = 35184372088832.0;  // 2^45
@@ -53,17 +52,21 @@ struct SampleBatch {
 
 typedef unsigned long long u64;
 
+// Logits as they are compared: NaN is -inf, -0 is 0.
+MF_DEVICE float sb_clean(float x) { return x != x ? -INFINITY : x + 0.0f; }
+// Order-preserving whole number of a clean value, and back.
 MF_DEVICE uint32_t sb_key(float x) {
-    if (x != x) x = -INFINITY;
-    const uint32_t u = __float_as_uint(x + 0.0f);  // -0 and 0 are equal
+    const uint32_t u = __float_as_uint(x);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 MF_DEVICE float sb_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
-// Level-1 bin of a value: never decreases as x falls.
+// Level-1 bin of a value, sixteenths below the top: never decreases as x falls.
+// (Rounded by the sum with 2^23, whose low bits are the whole number: a
+// conversion costs four times as much.)
 MF_DEVICE int sb_bin(float top, float x) {
-    const float d = x == top ? 0.f : top - x;  // top may be infinite
-    return d < (float)SB_BINS / 16.f ? (int)(d * 16.f) : SB_BINS - 1;
+    const float d = x == top ? 0.f : fminf(top - x, 31.95f);  // top may be infinite
+    return __float_as_int(fmaf(d, 16.f, 8388608.f)) - 0x4b000000;
 }
 
 MF_DEVICE uint32_t sb_remote(const void* local, int rank) {
@@ -82,6 +85,24 @@ MF_DEVICE u64 sb_ld64(const u64* local, int rank) {
     return v;
 }
 
+// Sum and maximum of a word over the blocks of the cluster. All loads are
+// issued before the first is used: one after the other costs a remote latency each.
+template <typename T> MF_DEVICE T sb_ld(const T* local, int rank) {
+    if constexpr (sizeof(T) == 8) return sb_ld64(local, rank);
+    else return sb_ld32(local, rank);
+}
+template <typename T> MF_DEVICE void sb_ld_all(const T* local, int size, T (&v)[SB_MAX_CLUSTER]) {
+#pragma unroll
+    for (int q = 0; q < SB_MAX_CLUSTER; ++q) v[q] = q < size ? sb_ld(local, q) : 0;
+}
+template <typename T> MF_DEVICE T sb_sum_all(const T* local, int size) {
+    T v[SB_MAX_CLUSTER], s = 0;
+    sb_ld_all(local, size, v);
+#pragma unroll
+    for (int q = 0; q < SB_MAX_CLUSTER; ++q) s += v[q];
+    return s;
+}
+
 // The last kept candidate of a prefix of the order.
 struct SbBorder {
     uint32_t key, idx;
@@ -90,27 +111,27 @@ struct SbBorder {
 };
 
 struct SbShared {
+    uint32_t cnt[SB_BINS];
+    uint32_t part[3][SB_BINS];  // weights in three parts of 16 bits: 32-bit shared atomics, no overflow below 2^16 terms
     union {
-        struct {
-            uint32_t cnt[SB_BINS];
-            uint32_t part[3][SB_BINS];  // weights in three parts of 16 bits: 32-bit shared atomics, no overflow below 2^16 terms
-            u64 wsum[SB_BINS];          // their sum, what the other blocks read
-        };
-        u64 sorted[SB_SORT];  // candidates of the whole row (its first block)
+        u64 wsum[SB_BINS];                   // their sum, what the other blocks read
+        float queue[SB_THREADS / 32][64];    // sb_scan_slice
     };
-    u64 cand[SB_SORT];          // (key, ~index) of the block's candidates
+    double table[256];          // 2^(-i / 256)
+    u64 cand[SB_FEW];          // (key, ~index) of the block's candidates
     u64 best;                   // (key, ~index) of the block's largest
     u64 scan[34];
-    uint32_t scan_c[32];
     u64 found[4];
     uint32_t list_n;
     uint32_t list_key[SB_LIST], list_idx[SB_LIST];
     uint32_t ties;
     uint32_t first;             // smallest position asked for
+    u64 sum[2];                 // the block's share of two sums, read by the others
+    u64 told[4];                // what the row's first block found
 };
 
 struct SbRow {
-    const uint32_t* keys;  // this block's slice
+    const float* vals;  // this block's slice
     int n, base;           // its length and first index
     int rank, size;        // of the cluster
     float top;
@@ -119,21 +140,41 @@ struct SbRow {
 
 enum SbMode { SB_COUNT, SB_WEIGHT };
 
-// Where a border falls among the level-1 bins of the whole row.
+// Where a border falls among the level-1 bins of the whole row, and the candidates up to the bin's end.
 struct SbLevel {
     int bin;
-    u64 before;     // running sum up to the bin
-    u64 total;      // over the prefix
-    uint32_t in_bin, upto;  // candidates in the bin, and up to its end
-    double target;
+    uint32_t upto;
 };
 
-// exp((x - top) / T) in multiples of 2^-45
-MF_DEVICE u64 sb_weight(float x, float top, double inv_t) {
+// exp((x - top) / T) in multiples of 2^-45, rounded to nearest. With z = top -
+// x and n = rint(256 z / (T ln 2)): exp(-z/T) = 2^-(n >> 8) * 2^-(n & 255)/256 *
+// e^t, t = n ln2/256 - z/T, |t| < 1.4e-3, where the series up to t^4/24 leaves
+// 4e-17 (a table and a short polynomial, Tang 1989). About half the 64-bit
+// operations of exp(); rows that keep most of the vocabulary spend their time here.
+struct SbTemp {
+    double inv_t, inv_step;  // 1 / T, 256 / (T ln 2)
+};
+MF_DEVICE SbTemp sb_temp(double t) {
+    SbTemp s;
+    s.inv_t = 1.0 / t;
+    s.inv_step = 369.3299304675746 * s.inv_t;  // 256 / ln 2
+    return s;
+}
+MF_DEVICE u64 sb_weight(float x, float top, const SbTemp& s, const double* table) {
     if (x == top) return (u64)SB_ONE;
-    const double z = ((double)x - (double)top) * inv_t;
-    if (!(z > -32.0)) return 0;  // below half of 2^-45
-    return (u64)(exp(z) * SB_ONE + 0.5);
+    const double z = (double)top - (double)x, e = z * s.inv_t;
+    if (!(e < 32.0)) return 0;  // below half of 2^-45
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52: the low bits of the sum are a whole number
+    const double kk = fma(z, s.inv_step, magic);
+    const int n = __double2loint(kk);
+    const double t = fma(kk - magic, 0.0027076061740622863, -e);  // ln 2 / 256
+    double p = fma(t, 1.0 / 24, 1.0 / 6);
+    p = fma(t, p, 0.5);
+    p = fma(t, p, 1.0);
+    p = fma(t, p, 1.0);
+    const double v = p * table[n & 255];  // in [0.49, 1.01)
+    const double w = __hiloint2double(__double2hiint(v) + (45 - (n >> 8)) * 1048576, __double2loint(v));
+    return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;  // + 2^52
 }
 
 // Block-wide inclusive scan of one u64 per thread.
@@ -157,40 +198,6 @@ MF_DEVICE u64 sb_scan(u64 v, SbShared* sh, u64& total) {
     return v + base;
 }
 
-// Inclusive scans of a u64 and a count per thread.
-MF_DEVICE u64 sb_scan2(u64 v, uint32_t& c, SbShared* sh, u64& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const u64 u = __shfl_up_sync(0xffffffffu, v, o);
-        const uint32_t d = __shfl_up_sync(0xffffffffu, c, o);
-        if (lane >= o) {
-            v += u;
-            c += d;
-        }
-    }
-    __syncthreads();
-    if (lane == 31) {
-        sh->scan[warp] = v;
-        sh->scan_c[warp] = c;
-    }
-    __syncthreads();
-    u64 base = 0;
-    uint32_t base_c = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < SB_THREADS / 32; ++w) {
-        const u64 x = sh->scan[w];
-        if (w < warp) {
-            base += x;
-            base_c += sh->scan_c[w];
-        }
-        total += x;
-    }
-    c += base_c;
-    return v + base;
-}
-
 // Smallest key of level-1 bin `bin` or below it in the order (monotone search).
 MF_DEVICE uint32_t sb_bin_low(float top, int bin) {
     uint32_t lo = sb_key(-INFINITY), hi = sb_key(top);  // bin(hi) = 0 <= bin
@@ -202,144 +209,233 @@ MF_DEVICE uint32_t sb_bin_low(float top, int bin) {
     return lo;
 }
 
-// Adds one candidate to a bin.
-template <int MODE> MF_DEVICE void sb_add(SbShared* sh, int bin, float x, float top, double inv_t) {
-    if (MODE == SB_WEIGHT) {
-        const u64 w = sb_weight(x, top, inv_t);
-        if (w) {
-            atomicAdd(&sh->part[0][bin], (uint32_t)(w & 0xffff));
-            atomicAdd(&sh->part[1][bin], (uint32_t)((w >> 16) & 0xffff));
-            atomicAdd(&sh->part[2][bin], (uint32_t)(w >> 32));
-        }
-    }
-    atomicAdd(&sh->cnt[bin], 1u);
-}
-
-// The bin in which the running sum over the prefix `in` reaches the target:
-// `want` ones, or share * (the sum) for weights. The block's bins must be zero
-// and in step (sb_clear). The same in every block of the cluster.
+// The block's bins at zero (in step before the first use).
 MF_DEVICE void sb_clear(SbShared* sh) {
     const int tid = threadIdx.x;
     sh->cnt[tid] = 0;
-    sh->part[0][tid] = sh->part[1][tid] = sh->part[2][tid] = 0;
+    sh->part[0][tid] = sh->part[1][tid] = 0;
     if (tid == 0) sh->first = ~0u;
 }
-template <int MODE>
-MF_DEVICE SbLevel sb_level(const SbRow& r, const SbBorder& in, double inv_t, u64 want, double share) {
+
+// The first thread with `hit` (SB_THREADS if none has); sh->first must be ~0 and in step. One call per use.
+MF_DEVICE int sb_first_thread(bool hit, SbShared* sh) {
+    const unsigned hits = __ballot_sync(0xffffffffu, hit);
+    if ((threadIdx.x & 31) == 0 && hits) atomicMin(&sh->first, threadIdx.x + __ffs(hits) - 1);
+    __syncthreads();
+    return min(sh->first, (uint32_t)SB_THREADS);
+}
+
+// The bin of the want-th candidate and the number of candidates up to its end.
+MF_DEVICE SbLevel sb_count_level(const SbRow& r, uint32_t want) {
     SbShared* sh = r.sh;
     const int tid = threadIdx.x;
-    const uint32_t whole = in.key == 0 ? 1 : 0;  // the prefix is everything
-    for (int i = tid; i < r.n; i += SB_THREADS) {
-        const uint32_t k = r.keys[i];
-        if (!whole && !in.keeps(k, r.base + i)) continue;
-        const float x = sb_value(k);
-        sb_add<MODE>(sh, sb_bin(r.top, x), x, r.top, inv_t);
-    }
-    __syncthreads();
-    if (MODE == SB_WEIGHT)
-        sh->wsum[tid] = (u64)sh->part[0][tid] + ((u64)sh->part[1][tid] << 16) + ((u64)sh->part[2][tid] << 32);
+    #pragma unroll 4
+    for (int i = tid; i < r.n; i += SB_THREADS) atomicAdd(&sh->cnt[sb_bin(r.top, r.vals[i])], 1u);
     cluster_sync_all();
-    uint32_t c = 0;
-    u64 w = 0;
-    for (int q = 0; q < r.size; ++q) {
-        c += sb_ld32(&sh->cnt[tid], q);
-        if (MODE == SB_WEIGHT) w += sb_ld64(&sh->wsum[tid], q);
-    }
-    if (MODE == SB_COUNT) w = c;
+    const uint32_t c = sb_sum_all(&sh->cnt[tid], r.size);
+    u64 total;
+    const u64 inc = sb_scan(c, sh, total);
     SbLevel v;
-    uint32_t upto = c;
-    const u64 inc = sb_scan2(w, upto, sh, v.total);
-    v.target = MODE == SB_COUNT ? (double)want : share * (double)v.total;
-    const bool hit = c > 0 && (double)inc >= v.target;
-    const unsigned hits = __ballot_sync(0xffffffffu, hit);
-    if ((tid & 31) == 0 && hits) atomicMin(&sh->first, (uint32_t)tid + __ffs(hits) - 1);
-    __syncthreads();
-    v.bin = sh->first;
-    if (tid == v.bin) {
-        sh->found[1] = inc - w;
-        sh->found[2] = (u64)upto << 32 | c;
-    }
+    v.bin = sb_first_thread(inc >= want, sh);
+    if (tid == v.bin) sh->found[0] = inc;
     cluster_sync_all();  // every block has read these bins
-    v.before = sh->found[1];
-    v.in_bin = (uint32_t)sh->found[2];
-    v.upto = (uint32_t)(sh->found[2] >> 32);
+    v.upto = (uint32_t)sh->found[0];
     return v;
 }
 
-// Brings the candidates with keys in [lo, hi] of the prefix `in` to the row's
-// first block and sorts them there (value, then index): n <= SB_SORT of them
-// in all. False in the other blocks, which have nothing more to do.
-MF_DEVICE bool sb_gather(const SbRow& r, const SbBorder& in, uint32_t lo, uint32_t hi, int n) {
-    SbShared* sh = r.sh;
-    const int tid = threadIdx.x;
-    if (tid == 0) sh->list_n = 0;
-    __syncthreads();
-    for (int i = tid; i < r.n; i += SB_THREADS) {
-        const uint32_t k = r.keys[i];
-        if (k < lo || k > hi || !in.keeps(k, r.base + i)) continue;
-        sh->cand[atomicAdd(&sh->list_n, 1u)] = (u64)k << 32 | (uint32_t)~(r.base + i);
-    }
-    cluster_sync_all();
-    if (r.rank == 0) {
-        int m = 32;
-        while (m < n) m *= 2;
-        int at = 0;
-        for (int q = 0; q < r.size; ++q) {
-            const int nq = sb_ld32(&sh->list_n, q);
-            for (int i = tid; i < nq; i += SB_THREADS) sh->sorted[at + i] = sb_ld64(&sh->cand[i], q);
-            at += nq;
-        }
-        for (int i = n + tid; i < m; i += SB_THREADS) sh->sorted[i] = 0;
-        __syncthreads();
-        for (int size = 2; size <= m; size *= 2)
-            for (int stride = size / 2; stride > 0; stride /= 2) {
-                for (int i = tid; i < m / 2; i += SB_THREADS) {
-                    const int x = 2 * i - (i & (stride - 1)), y = x + stride;
-                    const u64 u = sh->sorted[x], v = sh->sorted[y];
-                    if ((u < v) == ((x & size) == 0)) {
-                        sh->sorted[x] = v;
-                        sh->sorted[y] = u;
-                    }
-                }
-                __syncthreads();
-            }
-    }
-    cluster_sync_all();  // the lists have been read
-    return r.rank == 0;
+// Relative weight of a value within its bin, exp(-(z - (bin - 1/2)/16) / T), in 16
+// bits: sums of these tell (nearly always) in which bin an exact running sum
+// reaches its target, at one 32-bit atomic each instead of three exact ones.
+MF_DEVICE uint32_t sb_coarse(float top, float x, int bin, float c) {
+    const float d = x == top ? 0.f : top - x;
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(fmaf(-d, 16.f, (float)bin - 0.5f), 0.f) * c));
+    return (uint32_t)__float_as_int(fmaf(e, 65535.f, 8388608.f)) & 0x7fffffu;  // as in sb_bin
+}
+// The coarse weight of this thread's bin over the whole row, in multiples of
+// 2^-45 of the top's, from the blocks' sums in part[which].
+MF_DEVICE u64 sb_coarse_bin(const SbRow& r, int which, float c) {
+    uint32_t v[SB_MAX_CLUSTER];
+    sb_ld_all(&r.sh->part[which][threadIdx.x], r.size, v);
+    u64 w = 0;
+#pragma unroll
+    for (int q = 0; q < SB_MAX_CLUSTER; ++q) w += v[q];
+    return (u64)((double)w * exp2(-((double)threadIdx.x - 0.5) * c) * (SB_ONE / 65535.0));
 }
 
-// Position of the first of the n sorted candidates at which before + (running
-// sum of weights) reaches share * total, or target if share < 0; n - 1 if none
-// does. total 0: the sum over the n. Sets `sum` to that total.
-MF_DEVICE int sb_first(const SbRow& r, int n, double inv_t, u64 before, u64 total, double share, u64& sum) {
-    SbShared* sh = r.sh;
-    const int tid = threadIdx.x;
-    constexpr int E = SB_SORT / SB_THREADS;
-    u64 w[E], mine = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int i = tid * E + e;
-        w[e] = i < n ? sb_weight(sb_value((uint32_t)(sh->sorted[i] >> 32)), r.top, inv_t) : 0;
-        mine += w[e];
-    }
-    u64 all;
-    u64 run = before + sb_scan(mine, sh, all) - mine;
-    sum = total ? total : all;
-    const double target = share * (double)sum;
-    if (tid == 0) sh->first = n - 1;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        run += w[e];
-        if (tid * E + e < n && (double)run >= target) {
-            atomicMin(&sh->first, (uint32_t)(tid * E + e));
-            break;
+// Notes a candidate for sb_fetch (sh->list_n counts on past the end).
+MF_DEVICE void sb_note(SbShared* sh, uint32_t key, uint32_t idx) {
+    const uint32_t at = atomicAdd(&sh->list_n, 1u);
+    if (at < SB_FEW) sh->cand[at] = (u64)key << 32 | (uint32_t)~idx;
+}
+
+// Walks the block's slice and hands the values that `take` accepts to `add`, a
+// full warp of them at a time: few of many are accepted, and `add` is dear.
+template <typename Take, typename Add> MF_DEVICE void sb_scan_slice(const SbRow& r, Take take, Add add) {
+    const int lane = threadIdx.x & 31;
+    float* queue = r.sh->queue[threadIdx.x >> 5];
+    int n = 0;
+    for (int i0 = threadIdx.x & ~31; i0 < r.n; i0 += SB_THREADS) {
+        const int i = i0 + lane;
+        const float x = i < r.n ? r.vals[i] : 0.f;
+        const bool yes = i < r.n && take(x, i);
+        const unsigned who = __ballot_sync(0xffffffffu, yes);
+        if (yes) queue[n + __popc(who & ((1u << lane) - 1))] = x;
+        n += __popc(who);
+        if (n >= 32) {
+            __syncwarp();
+            add(queue[lane]);
+            __syncwarp();
+            n -= 32;
+            const float left = queue[32 + lane];
+            __syncwarp();
+            if (lane < n) queue[lane] = left;
         }
     }
+    __syncwarp();
+    if (lane < n) add(queue[lane]);
+    __syncwarp();
+}
+
+// Row's first block: the noted candidates of all blocks, four per thread (0:
+// none). Their number, or -1 if they are more than SB_FEW. The blocks are in
+// step before; they may leave after the next cluster barrier.
+constexpr int SB_E = SB_FEW / SB_THREADS;
+MF_DEVICE int sb_fetch(const SbRow& r, u64 (&v)[SB_E]) {
+    SbShared* sh = r.sh;
+    uint32_t nq[SB_MAX_CLUSTER];
+    sb_ld_all(&sh->list_n, r.size, nq);
+    uint32_t n = 0;
+#pragma unroll
+    for (int q = 0; q < SB_MAX_CLUSTER; ++q) n += nq[q];  // at most 2^18
+    if (n > SB_FEW) return -1;
+#pragma unroll
+    for (int e = 0; e < SB_E; ++e) {
+        uint32_t i = threadIdx.x + e * SB_THREADS;  // candidate i of all: i - (those of the blocks before) of block q
+        const bool in = i < n;
+        int q = 0;
+#pragma unroll
+        for (; q < SB_MAX_CLUSTER - 1; ++q) {
+            if (i < nq[q]) break;
+            i -= nq[q];
+        }
+        v[e] = in ? sb_ld64(&sh->cand[i], q) : 0;
+    }
+    return (int)n;
+}
+
+// sb_find among the fetched candidates of at least `cut`, by one block: the
+// first at which before + (running sum) reaches the target, `want` ones or
+// share * total (total 0: before + the sum over them, and set to that).
+// Candidates are distinct words (key, ~index), so the descent needs no rule
+// for ties. `right`: the border lies among them; the result counts only then.
+template <int MODE>
+MF_DEVICE u64 sb_pick(const SbRow& r, const u64 (&v)[SB_E], u64 cut, const SbTemp& t, u64 before, u64 want, double share,
+                      u64& total, bool& right) {
+    SbShared* sh = r.sh;
+    const int tid = threadIdx.x, lane = tid & 31;
+    u64 w[SB_E], lo = ~0ull, hi = 0;
+#pragma unroll
+    for (int e = 0; e < SB_E; ++e) {
+        const bool in = v[e] >= cut && v[e] != 0;
+        w[e] = !in ? 0 : MODE == SB_COUNT ? 1 : sb_weight(sb_value((uint32_t)(v[e] >> 32)), r.top, t, sh->table);
+        if (in) {
+            lo = min(lo, v[e]);
+            hi = max(hi, v[e]);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
     __syncthreads();
-    const int at = sh->first;
+    if (tid == 0) {
+        sh->found[0] = ~0ull;
+        sh->found[1] = 0;
+    }
     __syncthreads();
-    return at;
+    if (lane == 0) {
+        atomicMin(&sh->found[0], lo);
+        atomicMax(&sh->found[1], hi);
+    }
+    __syncthreads();
+    lo = sh->found[0];
+    hi = sh->found[1];
+    right = lo <= hi;
+    if (!right) return 0;
+    double target = (double)want;
+    for (int level = 0;; ++level) {
+        const int shift = max(64 - __clzll(hi - lo) - 9, 0);
+        sh->cnt[tid] = 0;
+        if (MODE == SB_WEIGHT) sh->part[0][tid] = sh->part[1][tid] = sh->part[2][tid] = 0;
+        if (tid == 0) {
+            sh->first = ~0u;
+            sh->list_n = 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < SB_E; ++e) {
+            if (v[e] < lo || v[e] > hi || v[e] < cut || v[e] == 0) continue;
+            const int bin = (int)((hi - v[e]) >> shift);
+            atomicAdd(&sh->cnt[bin], 1u);
+            if (MODE == SB_WEIGHT && w[e]) {
+                atomicAdd(&sh->part[0][bin], (uint32_t)(w[e] & 0xffff));
+                atomicAdd(&sh->part[1][bin], (uint32_t)((w[e] >> 16) & 0xffff));
+                atomicAdd(&sh->part[2][bin], (uint32_t)(w[e] >> 32));
+            }
+        }
+        __syncthreads();
+        const uint32_t c = sh->cnt[tid];
+        const u64 mine = MODE == SB_COUNT ? c : (u64)sh->part[0][tid] + ((u64)sh->part[1][tid] << 16) + ((u64)sh->part[2][tid] << 32);
+        u64 all;
+        const u64 inc = sb_scan(mine, sh, all);
+        if (level == 0) {
+            if (MODE == SB_WEIGHT) {
+                if (total == 0) total = before + all;
+                target = share * (double)total;
+            }
+            right = (before == 0 || (double)before < target) && (double)(before + all) >= target;
+            if (!right) return 0;
+        }
+        const int bin = sb_first_thread(c > 0 && (double)(before + inc) >= target, sh);
+        if (tid == bin) {
+            sh->found[1] = before + inc - mine;
+            sh->found[2] = c;
+        }
+        __syncthreads();
+        before = sh->found[1];
+        const uint32_t left = (uint32_t)sh->found[2];
+        hi -= (u64)bin << shift;
+        const u64 width = (1ull << shift) - 1;
+        if (hi - lo > width) lo = hi - width;
+        if (left <= 32) {
+            // one warp orders them: the largest at which the sum over those not below it reaches the target
+#pragma unroll
+            for (int e = 0; e < SB_E; ++e)
+                if (v[e] >= lo && v[e] <= hi && v[e] >= cut && v[e] != 0) {
+                    const uint32_t at = atomicAdd(&sh->list_n, 1u);
+                    sh->cand[at] = v[e];
+                    sh->wsum[at] = w[e];
+                }
+            __syncthreads();
+            if (tid < 32) {
+                const u64 x = lane < left ? sh->cand[lane] : 0, y = lane < left ? sh->wsum[lane] : 0;
+                u64 run = before;
+                for (uint32_t o = 0; o < left; ++o) {
+                    const u64 ox = __shfl_sync(0xffffffffu, x, o), oy = __shfl_sync(0xffffffffu, y, o);
+                    if (ox >= x) run += oy;
+                }
+                u64 best = lane < left && (double)run >= target ? x : 0;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+                if (lane == 0) sh->found[3] = best;
+            }
+            __syncthreads();
+            return sh->found[3];
+        }
+        __syncthreads();
+    }
 }
 
 // First candidate of the prefix `in` at which the running sum reaches the
@@ -348,7 +444,7 @@ MF_DEVICE int sb_first(const SbRow& r, int n, double inv_t, u64 before, u64 tota
 // cluster calls it and gets the same answer. If rounding leaves the target
 // above the sum the last candidate with weight is taken.
 template <int MODE>
-MF_DEVICE SbBorder sb_find(const SbRow& r, const SbBorder& in, double inv_t, u64 want, double share, u64& sum) {
+MF_DEVICE SbBorder sb_find(const SbRow& r, const SbBorder& in, const SbTemp& t, u64 want, double share, u64& sum) {
     SbShared* sh = r.sh;
     const int tid = threadIdx.x, lane = tid & 31;
     uint32_t lo = sb_key(-INFINITY), hi = sb_key(r.top);
@@ -365,13 +461,13 @@ MF_DEVICE SbBorder sb_find(const SbRow& r, const SbBorder& in, double inv_t, u64
         if (MODE == SB_WEIGHT) sh->part[0][tid] = sh->part[1][tid] = sh->part[2][tid] = 0;
         __syncthreads();
         for (int i = tid; i < r.n; i += SB_THREADS) {
-            const uint32_t k = r.keys[i];
+            const float x = r.vals[i];
+            const uint32_t k = sb_key(x);
             if (k < lo || k > hi || !in.keeps(k, r.base + i)) continue;
-            const float x = sb_value(k);
             const int bin = level == 0 ? sb_bin(r.top, x) : (int)((hi - k) >> shift);
             atomicAdd(&sh->cnt[bin], 1u);
             if (MODE == SB_WEIGHT) {
-                const u64 w = sb_weight(x, r.top, inv_t);
+                const u64 w = sb_weight(x, r.top, t, sh->table);
                 if (w) {
                     atomicAdd(&sh->part[0][bin], (uint32_t)(w & 0xffff));
                     atomicAdd(&sh->part[1][bin], (uint32_t)((w >> 16) & 0xffff));
@@ -383,13 +479,8 @@ MF_DEVICE SbBorder sb_find(const SbRow& r, const SbBorder& in, double inv_t, u64
         if (MODE == SB_WEIGHT)
             sh->wsum[tid] = (u64)sh->part[0][tid] + ((u64)sh->part[1][tid] << 16) + ((u64)sh->part[2][tid] << 32);
         cluster_sync_all();
-        uint32_t c = 0;
-        u64 w = 0;
-        for (int q = 0; q < r.size; ++q) {
-            c += sb_ld32(&sh->cnt[tid], q);
-            if (MODE == SB_WEIGHT) w += sb_ld64(&sh->wsum[tid], q);
-        }
-        if (MODE == SB_COUNT) w = c;
+        const uint32_t c = sb_sum_all(&sh->cnt[tid], r.size);
+        const u64 w = MODE == SB_WEIGHT ? sb_sum_all(&sh->wsum[tid], r.size) : c;
         u64 total;
         const u64 inc = sb_scan(w, sh, total);
         cluster_sync_all();  // every block has read these bins
@@ -437,7 +528,7 @@ MF_DEVICE SbBorder sb_find(const SbRow& r, const SbBorder& in, double inv_t, u64
                 if (tid == 0) sh->list_n = 0;
                 __syncthreads();
                 for (int i = tid; i < r.n; i += SB_THREADS) {
-                    const uint32_t k = r.keys[i];
+                    const uint32_t k = sb_key(r.vals[i]);
                     if (k < lo || k > hi || !in.keeps(k, r.base + i)) continue;
                     const uint32_t at = atomicAdd(&sh->list_n, 1u);
                     sh->list_key[at] = k;
@@ -463,7 +554,7 @@ MF_DEVICE SbBorder sb_find(const SbRow& r, const SbBorder& in, double inv_t, u64
                     u64 w2[2], run[2] = {0, 0};
                     uint32_t rank[2] = {0, 0};
                     for (int s = 0; s < 2; ++s)
-                        w2[s] = !has[s] ? 0 : MODE == SB_COUNT ? 1 : sb_weight(sb_value(k[s]), r.top, inv_t);
+                        w2[s] = !has[s] ? 0 : MODE == SB_COUNT ? 1 : sb_weight(sb_value(k[s]), r.top, t, sh->table);
                     for (int o = 0; o < 64; ++o) {  // rank and running sum by comparison with every candidate
                         const int src = o & 31, z = o >> 5;
                         const uint32_t ok = __shfl_sync(0xffffffffu, k[z], src), oi = __shfl_sync(0xffffffffu, ix[z], src);
@@ -492,8 +583,9 @@ MF_DEVICE SbBorder sb_find(const SbRow& r, const SbBorder& in, double inv_t, u64
                 out.key = (uint32_t)(sh->found[3] >> 32);
                 out.idx = (uint32_t)sh->found[3];
             } else {
+                const float one = sb_value(lo);
                 // one value: its ties in the order of their indices. Number `need` (from 1) is the border.
-                const u64 w1 = MODE == SB_COUNT ? 1 : sb_weight(sb_value(lo), r.top, inv_t);
+                const u64 w1 = MODE == SB_COUNT ? 1 : sb_weight(sb_value(lo), r.top, t, sh->table);
                 u64 need = left;
                 if (w1 > 0) {
                     u64 a = 1, z = left;  // smallest a with before + a * w1 >= target
@@ -509,7 +601,7 @@ MF_DEVICE SbBorder sb_find(const SbRow& r, const SbBorder& in, double inv_t, u64
                 const int seg = ((r.n + SB_THREADS - 1) / SB_THREADS) | 1;  // odd: a warp's runs start in different banks
                 const int i0 = min(tid * seg, r.n), i1 = min(i0 + seg, r.n);
                 uint32_t mine = 0;
-                for (int i = i0; i < i1; ++i) mine += r.keys[i] == lo && in.keeps(lo, r.base + i);
+                for (int i = i0; i < i1; ++i) mine += r.vals[i] == one && in.keeps(lo, r.base + i);
                 u64 all;
                 const u64 upto = sb_scan(mine, sh, all);
                 if (tid == 0) sh->ties = (uint32_t)all;
@@ -522,7 +614,7 @@ MF_DEVICE SbBorder sb_find(const SbRow& r, const SbBorder& in, double inv_t, u64
                 if (need > mine0 && need <= mine0 + mine) {
                     u64 left_n = need - mine0;
                     for (int i = i0; i < i1; ++i)
-                        if (r.keys[i] == lo && in.keeps(lo, r.base + i) && --left_n == 0) sh->found[3] = r.base + i;
+                        if (r.vals[i] == one && in.keeps(lo, r.base + i) && --left_n == 0) sh->found[3] = r.base + i;
                 }
                 cluster_sync_all();
                 out.key = lo;
@@ -539,8 +631,8 @@ MF_DEVICE SbBorder sb_find(const SbRow& r, const SbBorder& in, double inv_t, u64
 }
 
 template <typename T>
-__global__ void __launch_bounds__(SB_THREADS) sample_batch_kernel(const SampleBatch a) {
-    extern __shared__ __align__(16) uint32_t sb_keys[];
+__global__ void __launch_bounds__(SB_THREADS, 2) sample_batch_kernel(const SampleBatch a) {
+    extern __shared__ __align__(16) float sb_vals[];
     __shared__ SbShared sh;
     pdl_launch_dependents();
     pdl_wait();
@@ -553,12 +645,13 @@ __global__ void __launch_bounds__(SB_THREADS) sample_batch_kernel(const SampleBa
     r.size = size;
     r.base = r.rank * a.slice;
     r.n = max(min(a.slice, a.vocab - r.base), 0);
-    r.keys = sb_keys;
+    r.vals = sb_vals;
     r.sh = &sh;
 
-    // the slice as keys, and the largest with the lowest index
+    // the slice, and the largest with the lowest index
     const T* x = reinterpret_cast<const T*>(a.logits) + row * a.ld + r.base;
-    u64 best = 0;
+    float top = -INFINITY;
+    int at = -1;
     constexpr int V = 16 / sizeof(T);
     const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     const int nv = vec ? r.n / V : 0;
@@ -566,24 +659,35 @@ __global__ void __launch_bounds__(SB_THREADS) sample_batch_kernel(const SampleBa
         const PackV<T, V> v = *reinterpret_cast<const PackV<T, V>*>(x + (long long)i * V);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const uint32_t k = sb_key(to_f<T>(v.e[e]));
-            sb_keys[i * V + e] = k;
-            best = max(best, (u64)k << 32 | (uint32_t)~(r.base + i * V + e));
+            const float c = sb_clean(to_f<T>(v.e[e]));
+            sb_vals[i * V + e] = c;
+            if (c > top || at < 0) {
+                top = c;
+                at = i * V + e;
+            }
         }
     }
     for (int i = nv * V + tid; i < r.n; i += SB_THREADS) {
-        const uint32_t k = sb_key(to_f<T>(x[i]));
-        sb_keys[i] = k;
-        best = max(best, (u64)k << 32 | (uint32_t)~(r.base + i));
+        const float c = sb_clean(to_f<T>(x[i]));
+        sb_vals[i] = c;
+        if (c > top || at < 0) {
+            top = c;
+            at = i;
+        }
     }
+    u64 best = at < 0 ? 0 : (u64)sb_key(top) << 32 | (uint32_t)~(r.base + at);  // this thread saw its indices in order
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (tid == 0) sh.best = 0;
+    if (tid == 0) sh.best = sh.list_n = 0;
+    if (tid < 256) sh.table[tid] = exp2(-tid / 256.0);
     sb_clear(&sh);
     __syncthreads();
     if (lane == 0) atomicMax(&sh.best, best);
     cluster_sync_all();
+    u64 bests[SB_MAX_CLUSTER];
+    sb_ld_all(&sh.best, r.size, bests);
     best = 0;
-    for (int q = 0; q < r.size; ++q) best = max(best, sb_ld64(&sh.best, q));
+#pragma unroll
+    for (int q = 0; q < SB_MAX_CLUSTER; ++q) best = max(best, bests[q]);
     cluster_sync_all();
     const uint32_t top_key = (uint32_t)(best >> 32);
     r.top = sb_value(top_key);
@@ -594,65 +698,190 @@ __global__ void __launch_bounds__(SB_THREADS) sample_batch_kernel(const SampleBa
     const float temp = a.temp[row], top_p = a.top_p[row], min_p = a.min_p[row];
     const int top_k = a.top_k[row];
     const bool none = top_key == sb_key(-INFINITY);  // nothing to choose from
-    double prob = 1.0;
+    double prob = 1.0, inv_t = 1.0;
+    u64 sum = 0;
     if (!none && temp > 0.f) {
         const SbBorder all = {0u, ~0u};
         const bool cut_k = top_k > 0 && top_k < a.vocab, cut_p = top_p < 1.f;
-        const double share_p = (double)fmaxf(top_p, 0.f), inv_t = 1.0 / (double)temp;
-        const double draw = (double)fminf(fmaxf(a.draws[row], 0.f), 0.99999994f);
-        SbBorder likely = all;  // the smallest value at least min_p as likely as the first: x >= top + log(min_p)
+        const double share_p = (double)fmaxf(top_p, 0.f), draw = (double)fminf(fmaxf(a.draws[row], 0.f), 0.99999994f);
+        const SbTemp t1 = sb_temp(1.0), t2 = sb_temp((double)temp);
+        inv_t = t2.inv_t;
+        uint32_t low = 0;  // the smallest key at least min_p as likely as the first: x >= top + log(min_p)
         if (min_p > 0.f) {
             const double thr = min_p < 1.f ? (double)r.top + log((double)min_p) : (double)r.top;
-            uint32_t lo = sb_key(-INFINITY), hi = top_key;
-            while (lo < hi) {
-                const uint32_t mid = lo + ((hi - lo) >> 1);
-                if ((double)sb_value(mid) >= thr) hi = mid;
-                else lo = mid + 1;
-            }
-            likely.key = lo;
+            low = sb_key(__double2float_ru(thr));  // the smallest float that is not below thr
         }
-        u64 sum = 0;
-        bool done = false;
-        if (cut_k || cut_p) {
-            const SbLevel v = cut_k ? sb_level<SB_COUNT>(r, all, 1.0, (u64)top_k, -1.0) : sb_level<SB_WEIGHT>(r, all, 1.0, 0, share_p);
-            if (v.upto <= SB_SORT) {
-                // the candidates down to the bin of the first border: what is kept is among the first of them
-                if (!sb_gather(r, all, sb_bin_low(r.top, v.bin), top_key, (int)v.upto)) return;
-                int n = cut_k ? top_k : (int)v.upto;
-                if (cut_p) n = sb_first(r, n, 1.0, 0, cut_k ? 0 : v.total, share_p, sum) + 1;
-                if (min_p > 0.f) {
-                    if (tid == 0) sh.first = n;
-                    __syncthreads();
-                    for (int i = tid; i < n; i += SB_THREADS)
-                        if ((uint32_t)(sh.sorted[i] >> 32) < likely.key) atomicMin(&sh.first, (uint32_t)i);
-                    __syncthreads();
-                    n = sh.first;
-                    __syncthreads();
-                }
-                const u64 got = sh.sorted[sb_first(r, n, inv_t, 0, 0, draw, sum)];
+        bool done = false, right;
+        SbBorder kept = all;
+        if (cut_k) {
+            const SbLevel v = sb_count_level(r, (uint32_t)top_k);
+            if (v.upto <= SB_FEW) {
+                // few: the candidates down to the bin of the last go through the filters in order
+#pragma unroll 4
+                for (int i = tid; i < r.n; i += SB_THREADS)
+                    if (sb_bin(r.top, sb_vals[i]) <= v.bin) sb_note(&sh, sb_key(sb_vals[i]), r.base + i);
+                cluster_sync_all();
+                u64 v4[SB_E];
+                if (r.rank == 0) sb_fetch(r, v4);
+                cluster_sync_all();
+                if (r.rank != 0) return;
+                u64 part = 0, cut = sb_pick<SB_COUNT>(r, v4, 0, t1, 0, (u64)top_k, -1.0, part, right);
+                part = 0;
+                if (cut_p) cut = sb_pick<SB_WEIGHT>(r, v4, cut, t1, 0, 0, share_p, part, right);
+                if (low) cut = max(cut, (u64)low << 32);
+                const u64 got = sb_pick<SB_WEIGHT>(r, v4, cut, t2, 0, 0, draw, sum, right);
                 pick.key = (uint32_t)(got >> 32);
                 pick.idx = ~(uint32_t)got;
                 done = true;
+            } else {
+                kept = sb_find<SB_COUNT>(r, kept, t1, (u64)top_k, -1.0, sum);
+                if (cut_p) kept = sb_find<SB_WEIGHT>(r, kept, t1, 0, share_p, sum);
             }
         } else {
-            const SbLevel v = sb_level<SB_WEIGHT>(r, likely, inv_t, 0, draw);
-            if (v.in_bin <= SB_SORT) {
-                // the candidates of the draw's bin
-                const uint32_t lo = sb_bin_low(r.top, v.bin), hi = v.bin > 0 ? sb_bin_low(r.top, v.bin - 1) - 1 : top_key;
-                if (!sb_gather(r, likely, lo, hi, (int)v.in_bin)) return;
-                const u64 got = sh.sorted[sb_first(r, (int)v.in_bin, inv_t, v.before, v.total, draw, sum)];
-                pick.key = (uint32_t)(got >> 32);
-                pick.idx = ~(uint32_t)got;
-                done = true;
+            // Most of the vocabulary may be kept. One pass adds up the exact sum that the first target needs and,
+            // coarsely, the bins; then for each border one pass adds up what lies before its bin, exactly, and
+            // collects the bin.
+            const float c1 = 1.4426950408889634f / 16.f, c2 = (float)(1.4426950408889634 / 16 * t2.inv_t);
+            u64 s = 0;
+            const float low_x = low ? sb_value(low) : -INFINITY;
+            const bool same = temp == 1.f && !low;  // both borders have the same weights: one set of bins
+            if (cut_p) {
+#pragma unroll 2
+                for (int i = tid; i < r.n; i += SB_THREADS) {
+                    const float x = sb_vals[i];
+                    const int bin = sb_bin(r.top, x);
+                    s += sb_weight(x, r.top, t1, sh.table);
+                    atomicAdd(&sh.part[0][bin], sb_coarse(r.top, x, bin, c1));
+                    if (!same && x >= low_x) atomicAdd(&sh.part[1][bin], sb_coarse(r.top, x, bin, c2));
+                }
+            } else {
+#pragma unroll 2
+                for (int i = tid; i < r.n; i += SB_THREADS) {
+                    const float x = sb_vals[i];
+                    if (!(x >= low_x)) continue;
+                    const int bin = sb_bin(r.top, x);
+                    s += sb_weight(x, r.top, t2, sh.table);
+                    atomicAdd(&sh.part[1][bin], sb_coarse(r.top, x, bin, c2));
+                }
+            }
+            u64 block;
+            sb_scan(s, &sh, block);
+            if (tid == 0) sh.sum[0] = block;
+            cluster_sync_all();
+            sum = sb_sum_all(&sh.sum[0], r.size);
+            u64 w1 = 0, w2 = sb_coarse_bin(r, cut_p && same ? 0 : 1, c2), all1 = 0, all2;
+            if (cut_p) {
+                w1 = sb_coarse_bin(r, 0, c1);
+                w1 = sb_scan(w1, &sh, all1);
+            }
+            w2 = sb_scan(w2, &sh, all2);
+            cluster_sync_all();  // every block has read the bins and the sums
+            bool ok = true;
+            int last = SB_BINS - 1;  // the bin in which what is kept ends
+            if (cut_p) {
+                const int bin = sb_first_thread(w1 > 0 && (double)w1 >= share_p * (double)all1, &sh);
+                u64 s1 = 0, s2 = 0;
+                const bool same_t = temp == 1.f;
+                sb_scan_slice(r, [&](float x, int i) {
+                    const int b = sb_bin(r.top, x);
+                    if (b == bin) sb_note(&sh, sb_key(x), r.base + i);
+                    return b < bin;
+                }, [&](float x) {
+                    const u64 w = sb_weight(x, r.top, t1, sh.table);
+                    s1 += w;
+                    if (x >= low_x) s2 += same_t ? w : sb_weight(x, r.top, t2, sh.table);
+                });
+                u64 b1, b2;
+                sb_scan(s1, &sh, b1);
+                sb_scan(s2, &sh, b2);
+                if (tid == 0) {
+                    sh.sum[0] = b1;
+                    sh.sum[1] = b2;
+                }
+                cluster_sync_all();
+                if (r.rank == 0) {
+                    s1 = sb_sum_all(&sh.sum[0], r.size);
+                    s2 = sb_sum_all(&sh.sum[1], r.size);
+                    u64 v4[SB_E];
+                    ok = sb_fetch(r, v4) > 0;
+                    if (ok) {
+                        const u64 got = sb_pick<SB_WEIGHT>(r, v4, 0, t1, s1, 0, share_p, sum, right);
+                        ok = right;
+                        u64 weight = 0;  // of all that is kept
+                        if (ok) {        // the draw may fall into this bin
+                            const u64 g = sb_pick<SB_WEIGHT>(r, v4, max(got, (u64)low << 32), t2, s2, 0, draw, weight, right);
+                            if (weight == 0) weight = s2;  // nothing of the bin is kept
+                            sum = weight;
+                            if (right) {
+                                pick.key = (uint32_t)(g >> 32);
+                                pick.idx = ~(uint32_t)g;
+                                done = true;
+                            }
+                        }
+                        if (tid == 0) {
+                            sh.told[1] = got;
+                            sh.told[2] = sum;
+                        }
+                    }
+                    if (tid == 0) sh.told[0] = (ok ? 1u : 0u) | (done ? 2u : 0u);
+                }
+                cluster_sync_all();
+                const u64 told = sb_ld64(&sh.told[0], 0), got = sb_ld64(&sh.told[1], 0);
+                if (ok = told & 1; ok) sum = sb_ld64(&sh.told[2], 0);
+                done = told & 2;
+                cluster_sync_all();
+                if (done && r.rank != 0) return;
+                if (ok) {
+                    kept.key = (uint32_t)(got >> 32);
+                    kept.idx = ~(uint32_t)got;
+                    last = bin;
+                } else {
+                    kept = sb_find<SB_WEIGHT>(r, all, t1, 0, share_p, sum);
+                }
+                if (tid == 0) {
+                    sh.first = ~0u;
+                    sh.list_n = 0;
+                }
+                __syncthreads();
+            }
+            if (!done && ok) {
+                const int bin = min(sb_first_thread(w2 > 0 && (double)w2 >= draw * (double)sum, &sh), last);
+                u64 s2 = 0;
+                const float kept_x = kept.key ? sb_value(kept.key) : -INFINITY;
+                sb_scan_slice(r, [&](float x, int i) {
+                    if (!(x >= low_x) || x < kept_x || (x == kept_x && (uint32_t)(r.base + i) > kept.idx)) return false;
+                    const int b = sb_bin(r.top, x);
+                    if (b == bin) sb_note(&sh, sb_key(x), r.base + i);
+                    return b < bin;
+                }, [&](float x) { s2 += sb_weight(x, r.top, t2, sh.table); });
+                u64 b2;
+                sb_scan(s2, &sh, b2);
+                if (tid == 0) sh.sum[0] = b2;
+                cluster_sync_all();
+                if (r.rank == 0) {
+                    s2 = sb_sum_all(&sh.sum[0], r.size);
+                    u64 v4[SB_E];
+                    if (sb_fetch(r, v4) > 0) {
+                        const u64 got = sb_pick<SB_WEIGHT>(r, v4, 0, t2, s2, 0, draw, sum, right);
+                        if (right) {
+                            pick.key = (uint32_t)(got >> 32);
+                            pick.idx = ~(uint32_t)got;
+                            done = true;
+                        }
+                    }
+                    if (tid == 0) sh.told[0] = done ? 1 : 0;
+                }
+                cluster_sync_all();
+                done = sb_ld64(&sh.told[0], 0) != 0;
+                cluster_sync_all();
+                if (done && r.rank != 0) return;
             }
         }
         if (!done) {
-            // many candidates down to the border: filter by filter, by descent
-            SbBorder kept = all;
-            if (cut_k) kept = sb_find<SB_COUNT>(r, kept, 1.0, (u64)top_k, -1.0, sum);
-            if (cut_p) kept = sb_find<SB_WEIGHT>(r, kept, 1.0, 0, share_p, sum);
-            if (likely.before(kept)) kept = likely;
-            pick = sb_find<SB_WEIGHT>(r, kept, inv_t, 0, draw, sum);
+            // a crowded bin, or coarse sums that named the wrong one: the border of the draw by descent
+            const SbBorder likely = {low, ~0u};
+            if (low && likely.before(kept)) kept = likely;
+            pick = sb_find<SB_WEIGHT>(r, kept, t2, 0, draw, sum);
         }
         const float v = sb_value(pick.key);
         const double e = v == r.top ? 1.0 : exp(((double)v - (double)r.top) * inv_t);
