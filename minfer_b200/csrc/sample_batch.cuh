@@ -140,12 +140,6 @@ struct SbRow {
 
 enum SbMode { SB_COUNT, SB_WEIGHT };
 
-// Where a border falls among the level-1 bins of the whole row, and the candidates up to the bin's end.
-struct SbLevel {
-    int bin;
-    uint32_t upto;
-};
-
 // exp((x - top) / T) in multiples of 2^-45, rounded to nearest. With z = top -
 // x and n = rint(256 z / (T ln 2)): exp(-z/T) = 2^-(n >> 8) * 2^-(n & 255)/256 *
 // e^t, t = n ln2/256 - z/T, |t| < 1.4e-3, where the series up to t^4/24 leaves
@@ -225,22 +219,21 @@ MF_DEVICE int sb_first_thread(bool hit, SbShared* sh) {
     return min(sh->first, (uint32_t)SB_THREADS);
 }
 
-// The bin of the want-th candidate and the number of candidates up to its end.
-MF_DEVICE SbLevel sb_count_level(const SbRow& r, uint32_t want) {
+// A bin that ends at or behind the want-th candidate: the bin of the want-th
+// largest of the threads' maxima, since as many candidates are at least that
+// large. One atomic per thread instead of one per logit; with 4096 threads and
+// want up to 1000 hardly more than `want` candidates lie above its end.
+MF_DEVICE int sb_top_bin(const SbRow& r, bool has, float thread_max, uint32_t want) {
     SbShared* sh = r.sh;
     const int tid = threadIdx.x;
-    #pragma unroll 4
-    for (int i = tid; i < r.n; i += SB_THREADS) atomicAdd(&sh->cnt[sb_bin(r.top, r.vals[i])], 1u);
+    if (has) atomicAdd(&sh->cnt[sb_bin(r.top, thread_max)], 1u);
     cluster_sync_all();
     const uint32_t c = sb_sum_all(&sh->cnt[tid], r.size);
     u64 total;
     const u64 inc = sb_scan(c, sh, total);
-    SbLevel v;
-    v.bin = sb_first_thread(inc >= want, sh);
-    if (tid == v.bin) sh->found[0] = inc;
+    const int bin = sb_first_thread(inc >= want, sh);
     cluster_sync_all();  // every block has read these bins
-    v.upto = (uint32_t)sh->found[0];
-    return v;
+    return min(bin, SB_BINS - 1);
 }
 
 // Relative weight of a value within its bin, exp(-(z - (bin - 1/2)/16) / T), in 16
@@ -297,18 +290,20 @@ template <typename Take, typename Add> MF_DEVICE void sb_scan_slice(const SbRow&
     __syncwarp();
 }
 
-// Row's first block: the noted candidates of all blocks, four per thread (0:
-// none). Their number, or -1 if they are more than SB_FEW. The blocks are in
-// step before; they may leave after the next cluster barrier.
-constexpr int SB_E = SB_FEW / SB_THREADS;
-MF_DEVICE int sb_fetch(const SbRow& r, u64 (&v)[SB_E]) {
-    SbShared* sh = r.sh;
-    uint32_t nq[SB_MAX_CLUSTER];
-    sb_ld_all(&sh->list_n, r.size, nq);
+// Number of noted candidates of each block and of all. The blocks are in step before.
+MF_DEVICE uint32_t sb_noted(const SbRow& r, uint32_t (&nq)[SB_MAX_CLUSTER]) {
+    sb_ld_all(&r.sh->list_n, r.size, nq);
     uint32_t n = 0;
 #pragma unroll
     for (int q = 0; q < SB_MAX_CLUSTER; ++q) n += nq[q];  // at most 2^18
-    if (n > SB_FEW) return -1;
+    return n;
+}
+
+// Row's first block: the n <= SB_FEW noted candidates of all blocks, four per
+// thread (0: none). The blocks may leave after the next cluster barrier.
+constexpr int SB_E = SB_FEW / SB_THREADS;
+MF_DEVICE void sb_fetch(const SbRow& r, const uint32_t (&nq)[SB_MAX_CLUSTER], uint32_t n, u64 (&v)[SB_E]) {
+    SbShared* sh = r.sh;
 #pragma unroll
     for (int e = 0; e < SB_E; ++e) {
         uint32_t i = threadIdx.x + e * SB_THREADS;  // candidate i of all: i - (those of the blocks before) of block q
@@ -321,7 +316,6 @@ MF_DEVICE int sb_fetch(const SbRow& r, u64 (&v)[SB_E]) {
         }
         v[e] = in ? sb_ld64(&sh->cand[i], q) : 0;
     }
-    return (int)n;
 }
 
 // sb_find among the fetched candidates of at least `cut`, by one block: the
@@ -650,7 +644,7 @@ __global__ void __launch_bounds__(SB_THREADS, 2) sample_batch_kernel(const Sampl
 
     // the slice, and the largest with the lowest index
     const T* x = reinterpret_cast<const T*>(a.logits) + row * a.ld + r.base;
-    float top = -INFINITY;
+    float thread_max = -INFINITY;
     int at = -1;
     constexpr int V = 16 / sizeof(T);
     const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
@@ -661,8 +655,8 @@ __global__ void __launch_bounds__(SB_THREADS, 2) sample_batch_kernel(const Sampl
         for (int e = 0; e < V; ++e) {
             const float c = sb_clean(to_f<T>(v.e[e]));
             sb_vals[i * V + e] = c;
-            if (c > top || at < 0) {
-                top = c;
+            if (c > thread_max || at < 0) {
+                thread_max = c;
                 at = i * V + e;
             }
         }
@@ -670,12 +664,12 @@ __global__ void __launch_bounds__(SB_THREADS, 2) sample_batch_kernel(const Sampl
     for (int i = nv * V + tid; i < r.n; i += SB_THREADS) {
         const float c = sb_clean(to_f<T>(x[i]));
         sb_vals[i] = c;
-        if (c > top || at < 0) {
-            top = c;
+        if (c > thread_max || at < 0) {
+            thread_max = c;
             at = i;
         }
     }
-    u64 best = at < 0 ? 0 : (u64)sb_key(top) << 32 | (uint32_t)~(r.base + at);  // this thread saw its indices in order
+    u64 best = at < 0 ? 0 : (u64)sb_key(thread_max) << 32 | (uint32_t)~(r.base + at);  // this thread saw its indices in order
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     if (tid == 0) sh.best = sh.list_n = 0;
     if (tid < 256) sh.table[tid] = exp2(-tid / 256.0);
@@ -714,16 +708,29 @@ __global__ void __launch_bounds__(SB_THREADS, 2) sample_batch_kernel(const Sampl
         bool done = false, right;
         SbBorder kept = all;
         if (cut_k) {
-            const SbLevel v = sb_count_level(r, (uint32_t)top_k);
-            if (v.upto <= SB_FEW) {
-                // few: the candidates down to the bin of the last go through the filters in order
-#pragma unroll 4
-                for (int i = tid; i < r.n; i += SB_THREADS)
-                    if (sb_bin(r.top, sb_vals[i]) <= v.bin) sb_note(&sh, sb_key(sb_vals[i]), r.base + i);
-                cluster_sync_all();
-                u64 v4[SB_E];
-                if (r.rank == 0) sb_fetch(r, v4);
-                cluster_sync_all();
+            // few, as a rule: the candidates down to a bin that holds the last go through the filters in order
+            const int bin = sb_top_bin(r, at >= 0, thread_max, (uint32_t)top_k);
+            // (with a value for the bin's end, rounded down: one candidate more does no harm)
+            const float end = bin < SB_BINS - 1 ? __fsub_rd(r.top, ((float)bin + 0.51f) / 16.f) : -INFINITY;
+            const int n4 = r.n / 4;
+            for (int i = tid; i < n4; i += SB_THREADS) {
+                const float4 x = *reinterpret_cast<const float4*>(sb_vals + 4 * i);
+                if (fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= end) {
+                    if (x.x >= end) sb_note(&sh, sb_key(x.x), r.base + 4 * i);
+                    if (x.y >= end) sb_note(&sh, sb_key(x.y), r.base + 4 * i + 1);
+                    if (x.z >= end) sb_note(&sh, sb_key(x.z), r.base + 4 * i + 2);
+                    if (x.w >= end) sb_note(&sh, sb_key(x.w), r.base + 4 * i + 3);
+                }
+            }
+            for (int i = 4 * n4 + tid; i < r.n; i += SB_THREADS)
+                if (sb_vals[i] >= end) sb_note(&sh, sb_key(sb_vals[i]), r.base + i);
+            cluster_sync_all();
+            uint32_t nq[SB_MAX_CLUSTER];
+            const uint32_t n = sb_noted(r, nq);
+            u64 v4[SB_E];
+            if (r.rank == 0 && n <= SB_FEW) sb_fetch(r, nq, n, v4);
+            cluster_sync_all();
+            if (n <= SB_FEW) {
                 if (r.rank != 0) return;
                 u64 part = 0, cut = sb_pick<SB_COUNT>(r, v4, 0, t1, 0, (u64)top_k, -1.0, part, right);
                 part = 0;
@@ -802,9 +809,12 @@ __global__ void __launch_bounds__(SB_THREADS, 2) sample_batch_kernel(const Sampl
                 if (r.rank == 0) {
                     s1 = sb_sum_all(&sh.sum[0], r.size);
                     s2 = sb_sum_all(&sh.sum[1], r.size);
-                    u64 v4[SB_E];
-                    ok = sb_fetch(r, v4) > 0;
+                    uint32_t nq[SB_MAX_CLUSTER];
+                    const uint32_t n = sb_noted(r, nq);
+                    ok = n > 0 && n <= SB_FEW;
                     if (ok) {
+                        u64 v4[SB_E];
+                        sb_fetch(r, nq, n, v4);
                         const u64 got = sb_pick<SB_WEIGHT>(r, v4, 0, t1, s1, 0, share_p, sum, right);
                         ok = right;
                         u64 weight = 0;  // of all that is kept
@@ -860,8 +870,11 @@ __global__ void __launch_bounds__(SB_THREADS, 2) sample_batch_kernel(const Sampl
                 cluster_sync_all();
                 if (r.rank == 0) {
                     s2 = sb_sum_all(&sh.sum[0], r.size);
-                    u64 v4[SB_E];
-                    if (sb_fetch(r, v4) > 0) {
+                    uint32_t nq[SB_MAX_CLUSTER];
+                    const uint32_t n = sb_noted(r, nq);
+                    if (n > 0 && n <= SB_FEW) {
+                        u64 v4[SB_E];
+                        sb_fetch(r, nq, n, v4);
                         const u64 got = sb_pick<SB_WEIGHT>(r, v4, 0, t2, s2, 0, draw, sum, right);
                         if (right) {
                             pick.key = (uint32_t)(got >> 32);
