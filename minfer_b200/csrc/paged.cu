@@ -4,9 +4,12 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdlib>
+#include <map>
 #include <mutex>
+#include <utility>
 
 #include "minfer_cuda.h"
 #include "paged_attn.cuh"
@@ -47,12 +50,18 @@ cudaError_t launch(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStrea
 }
 
 int num_sms() {
+    static std::atomic<int> known[64];
     int dev = 0, v = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) {
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
         cudaGetLastError();
         return 148;
     }
+    if ((v = known[dev].load()) > 0) return v;
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) {
+        cudaGetLastError();
+        return 148;
+    }
+    known[dev] = v;
     return v;
 }
 
@@ -188,15 +197,24 @@ FewPlan few_plan(int dtype, int d, long long rows) {
     return dtype == MF_F16 ? mma_plan2<__half>(d, one) : mma_plan2<__nv_bfloat16>(d, one);
 }
 
-// Blocks of `fn` that are resident at once; also sets its shared-memory size.
+// Blocks of `fn` that are resident at once; also sets its shared-memory size
+// (always the same for one kernel). Asked of the driver once per device.
 int resident(const void* fn, int threads, size_t smem, int* blocks) {
     static std::mutex mu;
-    std::lock_guard<std::mutex> lk(mu);
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    int per = 0;
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, fn, threads, smem);
+    static std::map<std::pair<int, const void*>, int> known;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return fail(MF_E_CUDA, cudaGetErrorString(e));
-    *blocks = std::max(per, 1) * num_sms();
+    std::lock_guard<std::mutex> lk(mu);
+    int& n = known[{dev, fn}];
+    if (n == 0) {
+        int per = 0;
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, fn, threads, smem);
+        if (e != cudaSuccess) return fail(MF_E_CUDA, cudaGetErrorString(e));
+        n = std::max(per, 1) * num_sms();
+    }
+    *blocks = n;
     return MF_OK;
 }
 

@@ -4,6 +4,8 @@
 #include <algorithm>
 #include <cstdlib>
 #include <mutex>
+#include <set>
+#include <utility>
 
 #include "minfer_cuda.h"
 #include "sample_batch.cuh"
@@ -47,12 +49,18 @@ extern "C" int mf_sample_batch(int* ids, float* probs, const void* logits, int d
     a.probs = probs;
     a.vocab = vocab;
     a.slice = ((vocab + cluster - 1) / cluster + 7) / 8 * 8;  // 16-byte pieces of aligned rows
-    const size_t smem = (size_t)a.slice * sizeof(uint32_t);
+    const size_t smem = (size_t)a.slice * sizeof(float);
     {
         static std::mutex mu;
+        static std::set<std::pair<int, const void*>> set;  // per device and kernel, once
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
         std::lock_guard<std::mutex> lk(mu);
-        cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (mf::SB_MAX_VOCAB / mf::SB_MAX_CLUSTER) * (int)sizeof(uint32_t));
+        if (e == cudaSuccess && !set.count({dev, fn})) {
+            e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (mf::SB_MAX_VOCAB / mf::SB_MAX_CLUSTER) * (int)sizeof(float));
+            if (e == cudaSuccess) set.insert({dev, fn});
+        }
         if (e != cudaSuccess) return fail(MF_E_CUDA, cudaGetErrorString(e));
     }
     cudaLaunchConfig_t cfg = {};

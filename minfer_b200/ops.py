@@ -9,11 +9,13 @@ Every call raises MinferError on a non-zero status.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+from struct import Struct
 
 import torch
 
 from ._lib import (MF_BF16, MF_F16, MF_F32, MF_ROPE_LINEAR, MF_ROPE_NTK, MF_ROPE_PLAIN, MF_ROPE_YARN, check, cuda_lib,
-                   mf_attn_desc, mf_paged_attn_desc, mf_paged_kv, mf_paged_rope_desc)
+                   mf_attn_desc)
 
 _lib = cuda_lib()
 
@@ -180,62 +182,74 @@ def lm_head(logits, x, norm_w, eps: float, w, vocab: int, d_model: int, step_sta
 _CODES = {torch.float32: MF_F32, torch.float16: MF_F16, torch.bfloat16: MF_BF16}
 _SCALINGS = {"none": MF_ROPE_PLAIN, "linear": MF_ROPE_LINEAR, "ntk": MF_ROPE_NTK, "yarn": MF_ROPE_YARN}
 
+# The descriptions (mf_paged_kv, mf_paged_rope_desc, mf_paged_attn_desc) as packed bytes, native layout: a decode step
+# is short enough for the time of filling ctypes structures to count.
+_KV = Struct("@PPqqqPPPiiiiiiii")
+_ROPE = Struct("@PqPqiiiiiffPPPP0P")
+_ATTN = Struct("@PqPqiifiiiPN")
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # absent on builds without CUDA
 
-def _tensor(t: torch.Tensor, name: str, dtype, device, dims: int) -> int:
-    """Address of a CUDA tensor on `device` with the given dtype and rank; strides are the caller's business."""
-    if t.dtype is not dtype or t.dim() != dims or t.device != device:
-        raise ValueError(f"{name}: expected a {dims}-d {dtype} tensor on {device}, got {t.dim()}-d {t.dtype} on {t.device}")
+
+def _tensor(t: torch.Tensor, name: str, dtype, device: int, dims: int) -> int:
+    """Address of a tensor on CUDA device `device` with the given dtype and rank; strides are the caller's business."""
+    if t.dtype is not dtype or t.dim() != dims or t.get_device() != device:
+        raise ValueError(f"{name}: expected a {dims}-d {dtype} tensor on cuda:{device}, got {t.dim()}-d {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
-def _vector(t: torch.Tensor | None, name: str, dtype, device, n: int) -> int | None:
+def _vector(t: torch.Tensor | None, name: str, dtype, device: int, n: int) -> int:
     if t is None:
-        return None
-    p = _tensor(t, name, dtype, device, 1)
-    if t.shape[0] != n or (n > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name}: expected {n} contiguous elements")
-    return p
+        return 0
+    if t.dtype is not dtype or t.dim() != 1 or t.get_device() != device or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name}: expected {n} contiguous {dtype} elements on cuda:{device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, name: str, dtype, device, n: int, width: int) -> tuple[int, int]:
+def _rows(t: torch.Tensor, name: str, dtype, device: int, n: int, width: int) -> tuple[int, int]:
     """Address and row stride of n rows of `width` contiguous elements: [n, width], or [n, heads, d_head]."""
-    dims = t.dim()
+    shape = t.shape
+    dims = len(shape)
     p = _tensor(t, name, dtype, device, 3 if dims == 3 else 2)
-    shape, stride = t.shape, t.stride()
     inner = shape[1] if dims == 2 else shape[1] * shape[2]
-    if shape[0] != n or inner != width or stride[-1] != 1 or (dims == 3 and stride[1] != shape[2]):
-        raise ValueError(f"{name}: expected {n} rows of {width} contiguous elements, got {tuple(shape)} with strides {stride}")
-    return p, stride[0] if n > 1 else width
+    if t.is_contiguous():
+        if shape[0] == n and inner == width:
+            return p, width
+    else:
+        stride = t.stride()
+        if shape[0] == n and inner == width and stride[-1] == 1 and (dims == 2 or stride[1] == shape[2]):
+            return p, stride[0] if n > 1 else width
+    raise ValueError(f"{name}: expected {n} rows of {width} contiguous elements, got {tuple(shape)} with strides {t.stride()}")
 
 
-def _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens, device) -> mf_paged_kv:
-    dtype = k_pages.dtype
+def _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens) -> tuple[bytes, int, int, int, int]:
+    """The cache's packed description, its device, KV heads, head width and dtype code."""
+    dtype, device, shape = k_pages.dtype, k_pages.get_device(), k_pages.shape
     code = _CODES.get(dtype)
-    if code is None or k_pages.dim() != 4 or device.type != "cuda":
+    if code is None or len(shape) != 4 or device < 0:
         raise ValueError("k_pages: expected a CUDA tensor [n_pages, n_kv_heads, page_size, d_head] of float32, float16 or bfloat16")
-    kp = k_pages.data_ptr()
     vp = _tensor(v_pages, "v_pages", dtype, device, 4)
-    n_pages, heads, size, d = shape = k_pages.shape
+    n_pages, heads, size, d = shape
     strides = k_pages.stride()
     if v_pages.shape != shape or v_pages.stride() != strides or strides[3] != 1:
         raise ValueError("k_pages and v_pages: expected the same shape and strides, heads contiguous")
     table = _tensor(page_table, "page_table", torch.int32, device, 2)
     n_seqs, max_pages = page_table.shape
-    if max_pages > 1 and page_table.stride(1) != 1:
+    table_stride, inner = page_table.stride()
+    if max_pages > 1 and inner != 1:
         raise ValueError("page_table: expected contiguous rows")
-    return mf_paged_kv(kp, vp, strides[0], strides[1], strides[2], table,
-                       _vector(q_start, "q_start", torch.int32, device, n_seqs + 1),
-                       _vector(kv_lens, "kv_lens", torch.int32, device, n_seqs),
-                       page_table.stride(0) if n_seqs > 1 else max_pages, max_pages, n_pages, size, n_seqs, heads, d, code)
+    return _KV.pack(k_pages.data_ptr(), vp, strides[0], strides[1], strides[2], table,
+                    _vector(q_start, "q_start", torch.int32, device, n_seqs + 1),
+                    _vector(kv_lens, "kv_lens", torch.int32, device, n_seqs),
+                    table_stride if n_seqs > 1 else max_pages, max_pages, n_pages, size, n_seqs, heads, d, code), device, heads, d, code
 
 
-def _on(device, fn, *args) -> None:
-    """fn(*args, stream) on torch's current stream of `device`."""
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, _stream()))
+def _on(device: int, fn, *args) -> None:
+    """fn(*args, stream) on torch's current stream of CUDA device `device`."""
+    if torch.cuda.current_device() == device:
+        check(fn(*args, _raw_stream(device) or _CUDA_STREAM_LEGACY))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, _stream()))
+            check(fn(*args, _raw_stream(device) or _CUDA_STREAM_LEGACY))
 
 
 def rope_freqs(d_rot: int, base: float, scaling: str = "none", factor: float = 1.0, orig_ctx: float = 0.0,
@@ -260,24 +274,26 @@ def paged_rope_append(q_out, k_pages, v_pages, page_table, qkv, q_start, kv_lens
     view of [n_pages, page_size, n_kv_heads, d_head]); page_table: int32 [n_seqs, max_pages]; q_out: [n_tokens,
     n_heads, d_head] in the pages' dtype; qkv: [n_tokens, (n_heads + 2 n_kv_heads) * d_head]; freqs: float64
     [d_rot / 2] in turns per position (rope_freqs). Rows of no sequence, and the rest of the pages, stay as they are."""
-    device = k_pages.device
-    kv = _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens, device)
-    d, n = kv.d_head, qkv.shape[0]
+    kv, device, heads, d, _ = _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens)
+    n, half = qkv.shape[0], freqs.shape[0]
     q_width = q_out.shape[1] * (q_out.shape[2] if q_out.dim() == 3 else 1)
     x_code = _CODES.get(qkv.dtype)
     if x_code is None:
         raise ValueError(f"qkv: unsupported dtype {qkv.dtype}")
     q, q_stride = _rows(q_out, "q_out", k_pages.dtype, device, n, q_width)
-    x, x_stride = _rows(qkv, "qkv", qkv.dtype, device, n, q_width + 2 * kv.n_kv_heads * d)
+    x, x_stride = _rows(qkv, "qkv", qkv.dtype, device, n, q_width + 2 * heads * d)
     if q_width % d:
         raise ValueError("q_out: expected whole heads")
-    half = freqs.shape[0]
-    desc = mf_paged_rope_desc(q, q_stride, x, x_stride, x_code, n, q_width // d, 2 * half, interleaved, mscale, eps,
-                              _vector(freqs, "freqs", torch.float64, device, half),
-                              _vector(q_norm_w, "q_norm_w", torch.float32, device, d),
-                              _vector(k_norm_w, "k_norm_w", torch.float32, device, d),
-                              _vector(positions, "positions", torch.int32, device, n))
-    _on(device, _lib.mf_paged_rope_append, C.byref(kv), C.byref(desc))
+    desc = _ROPE.pack(q, q_stride, x, x_stride, x_code, n, q_width // d, 2 * half, interleaved, mscale, eps,
+                      _vector(freqs, "freqs", torch.float64, device, half), _vector(q_norm_w, "q_norm_w", torch.float32, device, d),
+                      _vector(k_norm_w, "k_norm_w", torch.float32, device, d), _vector(positions, "positions", torch.int32, device, n))
+    _on(device, _lib.mf_paged_rope_append, kv, desc)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device: int, *sizes: int) -> int:
+    with torch.cuda.device(device):
+        return int(_lib.mf_paged_attention_workspace_bytes(*sizes))
 
 
 def paged_attention_workspace_bytes(n_tokens: int, n_heads: int, n_kv_heads: int, d_head: int, dtype: torch.dtype) -> int:
@@ -290,20 +306,18 @@ def paged_attention(out, q, k_pages, v_pages, page_table, q_start, kv_lens, *, s
     arguments as in paged_rope_append, out and q [n_tokens, n_heads, d_head]. scale 0 means 1 / sqrt(d_head). max_new
     and max_len are hints: the most new tokens and the longest length of a sequence. workspace: a uint8 tensor of
     paged_attention_workspace_bytes, 256-byte aligned, not shared by overlapping calls; None takes one from torch."""
-    device = k_pages.device
-    kv = _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens, device)
-    n, d = q.shape[0], kv.d_head
+    kv, device, heads, d, code = _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens)
+    n = q.shape[0]
     width = q.shape[1] * (q.shape[2] if q.dim() == 3 else 1)
     qp, q_stride = _rows(q, "q", k_pages.dtype, device, n, width)
     op, o_stride = _rows(out, "out", k_pages.dtype, device, n, width)
     if width % d:
         raise ValueError("q: expected whole heads")
     if workspace is None:
-        need = _lib.mf_paged_attention_workspace_bytes(n, width // d, kv.n_kv_heads, d, kv.dtype)
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    desc = mf_paged_attn_desc(op, o_stride, qp, q_stride, n, width // d, scale, window, max_new, max_len,
-                              _tensor(workspace, "workspace", torch.uint8, device, 1), workspace.shape[0])
-    _on(device, _lib.mf_paged_attention, C.byref(kv), C.byref(desc))
+        workspace = torch.empty(_workspace_bytes(device, n, width // d, heads, d, code), dtype=torch.uint8, device=k_pages.device)
+    desc = _ATTN.pack(op, o_stride, qp, q_stride, n, width // d, scale, window, max_new, max_len,
+                      _tensor(workspace, "workspace", torch.uint8, device, 1), workspace.shape[0])
+    _on(device, _lib.mf_paged_attention, kv, desc)
 
 
 def paged_status(clear: bool = True) -> int:
@@ -317,15 +331,15 @@ def sample_batch(ids, logits, draws, temp, top_k, top_p, min_p, probs=None):
     """One id per row of logits [n_rows, vocab] (float32, float16 or bfloat16; rows may be strided): the reference
     Sampler's filters with row's own temp, top_k, top_p and min_p, and draws[row] in [0, 1) as its random number. ids and
     top_k are int32, the others float32 vectors of n_rows. probs (optional, float32) receives the ids' probabilities."""
-    device = logits.device
-    code = _CODES.get(logits.dtype)
-    if code is None or logits.dim() != 2 or device.type != "cuda":
+    device, code = logits.get_device(), _CODES.get(logits.dtype)
+    if code is None or logits.dim() != 2 or device < 0:
         raise ValueError("logits: expected a 2-d CUDA tensor of float32, float16 or bfloat16")
     n, vocab = logits.shape
-    if vocab > 1 and logits.stride(1) != 1:
+    stride, inner = logits.stride()
+    if vocab > 1 and inner != 1:
         raise ValueError("logits: expected contiguous rows")
-    f = torch.float32
-    _on(device, _lib.mf_sample_batch, _vector(ids, "ids", torch.int32, device, n), _vector(probs, "probs", f, device, n),
-        logits.data_ptr(), code, logits.stride(0) if n > 1 else vocab, n, vocab, _vector(draws, "draws", f, device, n),
-        _vector(temp, "temp", f, device, n), _vector(top_k, "top_k", torch.int32, device, n),
+    f, i = torch.float32, torch.int32
+    _on(device, _lib.mf_sample_batch, _vector(ids, "ids", i, device, n), _vector(probs, "probs", f, device, n),
+        logits.data_ptr(), code, stride if n > 1 else vocab, n, vocab, _vector(draws, "draws", f, device, n),
+        _vector(temp, "temp", f, device, n), _vector(top_k, "top_k", i, device, n),
         _vector(top_p, "top_p", f, device, n), _vector(min_p, "min_p", f, device, n))

@@ -141,3 +141,12 @@ def test_rope_freqs(d_rot, base):
 def test_bad_freqs(args):
     with pytest.raises(L.MinferError):
         ops.rope_freqs(*args)
+
+
+def test_packed_descriptions_match_the_structures():
+    """ops.py packs the C structures itself: same sizes and offsets as their ctypes declarations."""
+    for packed, struct in ((ops._KV, L.mf_paged_kv), (ops._ROPE, L.mf_paged_rope_desc), (ops._ATTN, L.mf_paged_attn_desc)):
+        assert packed.size == C.sizeof(struct)
+        values = [0.5 if t is C.c_float else i + 1 for i, (_, t) in enumerate(struct._fields_)]
+        got = struct.from_buffer_copy(packed.pack(*values))
+        assert [getattr(got, n) for n, _ in struct._fields_] == values
