@@ -97,22 +97,33 @@ EncodeFn tmap_encoder() {
     return encode;
 }
 
-// Largest power of two that divides page_size, at most `most`: keys of a page that one TMA box can bring in.
-int page_run(int page_size, int most) {
-    int r = page_size & -page_size;
-    return std::min(r, most);
-}
+// Keys of a page that one TMA box brings in: the largest power of two that divides page_size, at most 64.
+int page_run(int page_size) { return std::min(page_size & -page_size, 64); }
 
-// Map of 16-bit pages: (d, row of the page, head, page), boxes of 64 elements x `run` rows, 128-byte swizzle.
-int page_tmap(CUtensorMap* tm, const void* base, const mf::PagedKv& p, int D, int dtype, int run) {
+// Maps of the 16-bit pages: (d, row of the page, head, page, tensor), boxes of
+// 64 elements x `run` rows, 128-byte swizzle. One map serves K and V where their
+// distance can be its last stride (encoding a map takes about 3 us of host
+// time, a third of a decode call), else there are two. *at: K's index along the
+// last extent, and V's in bit 1.
+int page_tmaps(CUtensorMap* tk, CUtensorMap* tv, const mf::PagedKv& p, int D, int dtype, int run, int* at) {
     EncodeFn encode = tmap_encoder();
     if (!encode) return fail(MF_E_CUDA, "cuTensorMapEncodeTiled is not available");
-    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)p.page_size, (cuuint64_t)p.n_kv_heads, (cuuint64_t)p.n_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)p.row_stride * 2, (cuuint64_t)p.head_stride * 2, (cuuint64_t)p.page_stride * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)run, 1, 1}, es[4] = {1, 1, 1, 1};
-    const CUresult r = encode(tm, dtype == MF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                              const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    char *k = (char*)p.k, *v = (char*)p.v;
+    const cuuint64_t apart = k <= v ? (cuuint64_t)(v - k) : (cuuint64_t)(k - v);
+    const bool both = apart > 0 && apart < (1ull << 40);
+    *at = !both ? 0 : k < v ? 2 : 1;
+    const cuuint64_t dims[5] = {(cuuint64_t)D, (cuuint64_t)p.page_size, (cuuint64_t)p.n_kv_heads, (cuuint64_t)p.n_pages, both ? 2u : 1u};
+    const cuuint64_t strides[4] = {(cuuint64_t)p.row_stride * 2, (cuuint64_t)p.head_stride * 2, (cuuint64_t)p.page_stride * 2,
+                                   both ? apart : 16};
+    const cuuint32_t box[5] = {64, (cuuint32_t)run, 1, 1, 1}, es[5] = {1, 1, 1, 1, 1};
+    auto make = [&](CUtensorMap* tm, void* base) {
+        return encode(tm, dtype == MF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, base, dims,
+                      strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = make(tk, both ? std::min(k, v) : k);
+    if (both) *tv = *tk;
+    else if (r == CUDA_SUCCESS) r = make(tv, v);
     return r == CUDA_SUCCESS ? MF_OK : fail(MF_E_INVALID, "the pages' strides do not fit a tensor map");
 }
 
@@ -375,9 +386,16 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
     const bool chunks = kv->dtype != MF_F32 && (long long)most * G > FEW_ROWS;
     const bool few = !chunks || kv->n_seqs > 1;
     cudaError_t e = cudaSuccess;
+    CUtensorMap tk, tv;
+    int run = page_run(p.page_size), at = 0;
+    if (kv->dtype != MF_F32) {
+        rc = page_tmaps(&tk, &tv, p, D, kv->dtype, run, &at);
+        if (rc) return rc;
+    }
     if (chunks) {
         mf::PagedFa f = {};
-        f.run = page_run(p.page_size, mf::PF_KT);
+        f.run = run;
+        f.at = at;
         f.min_rows = few ? FEW_ROWS : 0;
         a.max_rows = few ? FEW_ROWS : 0;
         f.n_split = chunk_split(d->n_tokens, d->n_heads, kv->n_kv_heads);
@@ -385,10 +403,6 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
         const size_t rows = (size_t)d->n_tokens * d->n_heads;
         f.part_o = a.part + (mf_paged_attention_workspace_bytes(d->n_tokens, d->n_heads, kv->n_kv_heads, D, MF_F32) + 3) / 4;
         f.part_ml = (float2*)(f.part_o + f.n_split * rows * D);
-        CUtensorMap tk, tv;
-        rc = page_tmap(&tk, p.k, p, D, kv->dtype, f.run);
-        if (!rc) rc = page_tmap(&tv, p.v, p, D, kv->dtype, f.run);
-        if (rc) return rc;
         const void* fn = fa_fn(kv->dtype, D, false);
         const size_t smem = D == 64 ? mf::pf_smem<64>() : mf::pf_smem<128>();
         int unused = 0;
@@ -415,12 +429,7 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
             void* args[] = {&p, &a};
             e = launch(s.kernel, dim3(blocks), dim3(s.threads), s.smem, st, args);
         } else {
-            int run = page_run(p.page_size, D == 64 ? mf::pw_kt<64>() : mf::pw_kt<128>());
-            CUtensorMap tk, tv;
-            rc = page_tmap(&tk, p.k, p, D, kv->dtype, run);
-            if (!rc) rc = page_tmap(&tv, p.v, p, D, kv->dtype, run);
-            if (rc) return rc;
-            void* args[] = {&tk, &tv, &p, &a, &run};
+            void* args[] = {&tk, &tv, &p, &a, &run, &at};
             e = launch(s.kernel, dim3(blocks), dim3(s.threads), s.smem, st, args);
         }
         if (e == cudaSuccess && blocks > 1) {

@@ -70,12 +70,12 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
     float* l_s = alpha_s + RT;
     int* valid = reinterpret_cast<int*>(l_s + RT);
     __shared__ long long sh[34];
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();  // after the wait: see paged_join_kernel
 
     PagedItem it;
     long long share;
-    const long long total = paged_find<RT, KT>(p, a, blockIdx.x, true, gridDim.x, sh, share, it);
+    const long long total = paged_find<RT, KT>(p, a, blockIdx.x, gridDim.x, sh, share, it);
     const long long w0 = blockIdx.x * share, w1 = min(w0 + share, total);
     if (w0 >= w1) return;
 

@@ -49,6 +49,7 @@ template <int D> constexpr int pf_smem() { return (2 * PF_STAGES + 2) * pf_tile<
 
 struct PagedFa {
     int run;        // R: keys per TMA box
+    int at;         // K's index along the maps' last extent, and V's in bit 1
     int min_rows;   // sequences of at most this many rows are another kernel's
     int n_split;    // gridDim.y: shares of the key tiles
     float* part_o;  // n_split > 1: [split][n_tokens * n_heads][D], unnormalised
@@ -68,11 +69,12 @@ MF_DEVICE uint64_t pf_desc_rows_k(uint32_t saddr) {
     return d;
 }
 
-MF_DEVICE void tma_load_4d(void* dst, const CUtensorMap* tm, uint64_t* bar, int x, int y, int z, int w) {
+// One box of the pages' map (d, row of the page, head, page, tensor).
+MF_DEVICE void tma_load_page(void* dst, const CUtensorMap* tm, uint64_t* bar, int d, int row, int head, int page, int which) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::
             "r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(bar)), "r"(d), "r"(row), "r"(head), "r"(page), "r"(which)
         : "memory");
 }
 
@@ -183,6 +185,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (warp == 9 || warp == 10) {
             const bool is_k = warp == 9;
             const CUtensorMap* tm = is_k ? &tk : &tv;
+            const int which = is_k ? f.at & 1 : f.at >> 1;
             uint8_t* ring = is_k ? ks : vs;
             uint64_t* full = is_k ? k_full : v_full;
             uint64_t* free_ = is_k ? k_free : v_free;
@@ -225,7 +228,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                 if (whole) {
                     const int off = c0 % p.page_size;
 #pragma unroll
-                    for (int x = 0; x < D / 64; ++x) tma_load_4d(dst + x * PF_HALF + lane * R * 128, tm, &full[st], 64 * x, off, h, page);
+                    for (int x = 0; x < D / 64; ++x) tma_load_page(dst + x * PF_HALF + lane * R * 128, tm, &full[st], 64 * x, off, h, page, which);
                 }
                 issued = j + 1;
             }

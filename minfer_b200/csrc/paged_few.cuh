@@ -60,7 +60,7 @@ template <> MF_DEVICE void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], 
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(PW_THREADS, 2)
     paged_few_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const PagedKv p,
-                     const PagedAttn a, const int run) {
+                     const PagedAttn a, const int run, const int at) {
     constexpr int RT = 16 * MT, ST = pw_stages<MT>(), KT = pw_kt<D>(), TILE = pw_tile<D>(), HALF = KT * 128;
     constexpr int KW = KT / PW_WARPS;  // keys of one warp: 16 or 32
     extern __shared__ uint8_t pw_smem_raw[];
@@ -80,11 +80,12 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();  // after the wait: see paged_join_kernel
+    __syncthreads();
     PagedItem it;
     long long share;
-    const long long total = paged_find<RT, KT>(p, a, blockIdx.x, true, gridDim.x, sh, share, it);
+    const long long total = paged_find<RT, KT>(p, a, blockIdx.x, gridDim.x, sh, share, it);
     const long long w0 = blockIdx.x * share, w1 = min(w0 + share, total);
     if (w0 >= w1) return;
     const unsigned long long deadline = globaltimer_ns() + a.timeout_ns;
@@ -96,10 +97,10 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
         for (long long w = w0; w < w1 && !failed;) {
             const int j0 = (int)max(w - it.start, 0ll), j1 = (int)min((long long)it.tiles, w1 - it.start);
             if (j1 <= 0) break;  // only the item's first unit is in this range
-            const int k_first = it.k.lo / KT * KT;
+            const int key0 = it.k.lo / KT * KT;
             for (int j = j0; j < j1; ++j, ++n) {
                 const int st = n % ST;
-                const int c0 = k_first + j * KT + lane * R;  // this lane's run: keys [c0, c0 + R)
+                const int c0 = key0 + j * KT + lane * R;  // this lane's run: keys [c0, c0 + R)
                 const int page = lane < nr && c0 < it.k.hi && c0 + R > it.k.lo ? paged_page(p, it.b, c0) : -1;
                 const int off = c0 % p.page_size;
                 const unsigned boxes = __ballot_sync(0xffffffffu, page >= 0);
@@ -118,8 +119,8 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                 if (page >= 0) {
 #pragma unroll
                     for (int x = 0; x < D / 64; ++x) {
-                        tma_load_4d(kd + x * HALF + lane * R * 128, &tk, &full[st], 64 * x, off, it.h, page);
-                        tma_load_4d(vd + x * HALF + lane * R * 128, &tv, &full[st], 64 * x, off, it.h, page);
+                        tma_load_page(kd + x * HALF + lane * R * 128, &tk, &full[st], 64 * x, off, it.h, page, at & 1);
+                        tma_load_page(vd + x * HALF + lane * R * 128, &tv, &full[st], 64 * x, off, it.h, page, at >> 1);
                     }
                 }
             }
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
             const int j0 = (int)max(w - it.start, 0ll), j1 = (int)min((long long)it.tiles, w1 - it.start);
             if (j1 <= 0) break;  // only the item's first unit is in this range
             const int rows = min(RT, it.s.n * a.G - it.r0);
-            const int k_first = it.k.lo / KT * KT;
+            const int key0 = it.k.lo / KT * KT;
             const T* qb = reinterpret_cast<const T*>(a.q) + (long long)it.s.row * a.q_stride + (long long)it.h * a.G * D;
             auto q_row = [&](int r) { return qb + (long long)((it.r0 + r) / a.G) * a.q_stride + (long long)((it.r0 + r) % a.G) * D; };
             uint32_t qf[MT == 1 ? D / 16 : 1][4];
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                 const int st = n % ST;
                 mbar_wait(&full[st], (uint32_t)(n / ST) & 1u, deadline, failed);
                 const uint32_t kd = smem_u32(smem + st * 2 * TILE), vd = kd + TILE;
-                const int kw = KW * warp, k0 = k_first + j * KT + kw;  // this warp's keys
+                const int kw = KW * warp, k0 = key0 + j * KT + kw;  // this warp's keys
                 float s[MT][KW / 8][4];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)

@@ -64,16 +64,23 @@ struct PagedItem {
     PagedSpan k;
 };
 
-// Total work, and the item that holds unit `at` (if at < total). Called by the
-// whole block (a multiple of 32 threads, <= 1024); `sh` is shared scratch of 34
-// long longs. Each thread sums a run of sequences; the owner of `at` is found
-// in the block's prefix sums and walked by every thread.
+// a / b for a >= 0, b > 0; nearly always both are small, and a 64-bit division is five times as long
+MF_DEVICE long long paged_div(long long a, long long b) {
+    return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+
+// Total work, and the item that holds unit `at` (if at < total); at = n * share
+// with share = ceil(total / grid). Called by the whole block (a multiple of 32
+// threads, <= 1024); `sh` is shared scratch of 34 long longs. Each thread sums
+// a run of sequences; the owner of `at` is found in the prefix sums (each warp's
+// own for up to 32 sequences, else the block's) and walked by every thread.
 template <int RT, int KT>
-MF_DEVICE long long paged_find(const PagedKv& p, const PagedAttn& a, long long at_cta, bool as_share, int grid,
-                               long long* sh, long long& share, PagedItem& it) {
+MF_DEVICE long long paged_find(const PagedKv& p, const PagedAttn& a, int n, int grid, long long* sh, long long& share,
+                               PagedItem& it) {
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
-    const int run = (p.n_seqs + nt - 1) / nt;
-    const int b0 = min(tid * run, p.n_seqs), b1 = min(b0 + run, p.n_seqs);
+    const bool one = p.n_seqs <= 32;
+    const int run = one ? 1 : (p.n_seqs + nt - 1) / nt;
+    const int b0 = min((one ? lane : tid) * run, p.n_seqs), b1 = min(b0 + run, p.n_seqs);
     long long mine = 0;
     for (int b = b0; b < b1; ++b) mine += (long long)p.n_kv_heads * paged_head_work<RT, KT>(paged_seq(p, b), a);
     long long inc = mine;
@@ -82,34 +89,48 @@ MF_DEVICE long long paged_find(const PagedKv& p, const PagedAttn& a, long long a
         const long long v = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += v;
     }
-    if (lane == 31) sh[warp] = inc;
-    __syncthreads();
     long long base = 0, total = 0;
-    for (int w = 0; w < (nt >> 5); ++w) {
-        const long long v = sh[w];
-        if (w < warp) base += v;
-        total += v;
+    if (one) {
+        total = __shfl_sync(0xffffffffu, inc, 31);
+    } else {
+        if (lane == 31) sh[warp] = inc;
+        __syncthreads();
+        for (int w = 0; w < (nt >> 5); ++w) {
+            const long long v = sh[w];
+            if (w < warp) base += v;
+            total += v;
+        }
     }
-    share = (total + grid - 1) / grid;
-    const long long at = as_share ? at_cta * share : at_cta;
+    share = paged_div(total + grid - 1, grid);
+    const long long at = n * share;
     const long long begin = base + inc - mine;
-    __syncthreads();
-    if (mine > 0 && at >= begin && at < begin + mine) {
-        sh[32] = begin;
-        sh[33] = b0;
-    }
-    __syncthreads();
+    const bool here = mine > 0 && at >= begin && at < begin + mine;
+    long long w = begin;
+    int b = b0;
     it.tiles = 0;
-    if (at >= total) return total;
-    long long w = sh[32];
-    int b = (int)sh[33];
+    if (one) {
+        const unsigned who = __ballot_sync(0xffffffffu, here);
+        if (at >= total) return total;
+        const int src = __ffs(who) - 1;
+        w = __shfl_sync(0xffffffffu, w, src);
+        b = __shfl_sync(0xffffffffu, b, src);
+    } else {
+        if (here) {
+            sh[32] = begin;
+            sh[33] = b0;
+        }
+        __syncthreads();
+        if (at >= total) return total;
+        w = sh[32];
+        b = (int)sh[33];
+    }
     for (;; ++b) {
         const PagedSeq s = paged_seq(p, b);
         const int hw = paged_head_work<RT, KT>(s, a);
         if (hw > 0 && at < w + (long long)hw * p.n_kv_heads) {
             it.b = b;
             it.s = s;
-            it.h = (int)((at - w) / hw);
+            it.h = (int)paged_div(at - w, hw);
             w += (long long)it.h * hw;
             break;
         }
@@ -142,44 +163,62 @@ template <int RT, int KT> MF_DEVICE void paged_next(const PagedKv& p, const Page
     it.tiles = paged_tiles<KT>(it.k);
 }
 
-// Joins the parts of every item that a cut divides: block c (1 .. grid - 1)
-// takes the item whose first inner cut is c. Row by row, with m the largest
+// Joins the parts of every item that a cut divides: block c - 1 takes the item
+// whose first inner cut is c (1 .. grid - 1). Row by row, with m the largest
 // part maximum, out = sum O_i 2^(m_i - m) / sum l_i 2^(m_i - m). A part that
 // saw no key has m = -inf and adds nothing; a row without any key is 0.
+// The search for the item runs before the wait for the kernel that leaves the
+// parts: that kernel lets this one start only after its own wait, so the
+// batch's lengths are there.
 template <typename T, int D, int RT, int KT>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedKv p, const PagedAttn a, int grid) {
     __shared__ long long sh[34];
     pdl_launch_dependents();
-    pdl_wait();
     PagedItem it;
     long long share;
-    const long long c = (long long)blockIdx.x + 1;
-    const long long total = paged_find<RT, KT>(p, a, c, true, grid, sh, share, it);
+    const int c = (int)blockIdx.x + 1;
+    const long long total = paged_find<RT, KT>(p, a, c, grid, sh, share, it);
     const long long at = c * share;
-    if (at >= total || at <= it.start || it.start / share + 1 != c) return;
-    const int last = (int)((it.start + it.tiles - 1) / share);
-    const int first = (int)c - 1;
+    const bool mine = at < total && at > it.start && paged_div(it.start, share) + 1 == c;
+    const int last = mine ? (int)paged_div(it.start + it.tiles - 1, share) : 0;
+    pdl_wait();
+    if (!mine) return;
     const int rows = min(RT, it.s.n * a.G - it.r0);
     const float* ml = a.part + (long long)2 * grid * RT * D;
-    constexpr int V = D / 32;
+    constexpr int V = D / 32, U = 8;
     const int lane = threadIdx.x & 31;
+    // a CTA's slot 0 is for the item that its range begins inside of, slot 1 for the one it ends inside of:
+    // the parts are slot 1 of CTA c - 1 and slot 0 of the CTAs c .. last
+    const int n = last - c + 2;
     for (int r = threadIdx.x >> 5; r < rows; r += blockDim.x >> 5) {
-        // a CTA's slot 0 is for the item that its range begins inside of, slot 1 for the one it ends inside of
-        const int slot0 = 2 * first + 1;
         float m = -INFINITY;
-        for (int i = first; i <= last; ++i) m = fmaxf(m, __ldcg(ml + ((long long)(i == first ? slot0 : 2 * i) * RT + r) * 2));
+        for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(ml + ((long long)(2 * (c - 1 + i) + (i == 0)) * RT + r) * 2));
+        m = warp_max(m);
         float l = 0.f, o[V] = {};
-        if (m != -INFINITY) {
-            for (int i = first; i <= last; ++i) {
-                const long long at_r = (long long)(i == first ? slot0 : 2 * i) * RT + r;
-                const float2 v = __ldcg(reinterpret_cast<const float2*>(ml) + at_r);
-                const float w = v.x == -INFINITY ? 0.f : exp2f(v.x - m);
+        for (int i0 = 0; i0 < n && m != -INFINITY; i0 += 32) {
+            float w = 0.f;  // weight of part i0 + lane
+            if (i0 + lane < n) {
+                const int i = i0 + lane;
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(ml) + (long long)(2 * (c - 1 + i) + (i == 0)) * RT + r);
+                w = v.x == -INFINITY ? 0.f : exp2f(v.x - m);
                 l = fmaf(v.y, w, l);
-                const PackV<float, V> x = *reinterpret_cast<const PackV<float, V>*>(a.part + at_r * D + lane * V);
+            }
+            for (int i1 = 0; i1 < min(32, n - i0); i1 += U) {  // U loads in flight
+                PackV<float, V> x[U];
 #pragma unroll
-                for (int e = 0; e < V; ++e) o[e] = w != 0.f ? fmaf(x.e[e], w, o[e]) : o[e];
+                for (int u = 0; u < U; ++u) {
+                    const int i = min(i0 + i1 + u, n - 1);
+                    x[u] = *reinterpret_cast<const PackV<float, V>*>(a.part + ((long long)(2 * (c - 1 + i) + (i == 0)) * RT + r) * D + lane * V);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float wu = __shfl_sync(0xffffffffu, w, i1 + u);  // 0 past the last
+#pragma unroll
+                    for (int e = 0; e < V; ++e) o[e] = wu != 0.f ? fmaf(x[u].e[e], wu, o[e]) : o[e];
+                }
             }
         }
+        l = warp_sum(l);
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         PackV<T, V> y;
 #pragma unroll

@@ -163,6 +163,19 @@ def test_long_context():
     check_attention(b)
 
 
+@pytest.mark.parametrize("dtype", [t for t, _ in TYPES], ids=[n for _, n in TYPES])
+def test_k_and_v_in_one_tensor(dtype):
+    """K and V interleaved page by page in one allocation, V before K, and the same pages for both."""
+    b = ref.Batch([(1, 150), (40, 90)], 8, 2, 128, 16, dtype, seed=14)
+    q = b.q()
+    want = check_attention(b, q)
+    both = torch.stack([b.v, b.k], 1)  # [n_pages, 2, heads, page, d]
+    b.v, b.k = both[:, 0], both[:, 1]
+    assert torch.equal(run_attention(b, q), want)
+    b.v = b.k
+    check_attention(b, q)
+
+
 def test_many_sequences():
     seqs = [((i % 3 == 0) + (i % 50 == 7) * 20, 1 + (i * 37) % 300) for i in range(600)]
     seqs = [(min(n, length), length) for n, length in seqs]
