@@ -56,17 +56,41 @@ struct PagedFa {
     float2* part_ml;  // [split][n_tokens * n_heads]
 };
 
-// Shared-memory descriptor of an operand whose rows (128 bytes, 128-byte
-// swizzle) run along K: the next 8 rows 1024 bytes on, the next 64 elements of
-// the other extent PF_HALF bytes on.
-MF_DEVICE uint64_t pf_desc_rows_k(uint32_t saddr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-    d |= (uint64_t)((PF_HALF >> 4) & 0x3FFF) << 16;
-    d |= (uint64_t)((1024 >> 4) & 0x3FFF) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
+// Shared-memory descriptors of 128-byte-swizzled tiles. Their upper words are
+// constants and the address is the lowest field, so an operand a few 16-byte
+// units on is one 32-bit addition: a descriptor built anew for every MMA cost
+// as long as the MMA.
+//   PF_DESC_MN: rows run along the M or N extent (sw128_kmajor_desc): the next 8 rows 1024 bytes on.
+//   PF_DESC_K:  rows run along K: the next 8 rows 1024 bytes on, the next 64 elements of N PF_HALF bytes on.
+constexpr uint32_t PF_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+MF_DEVICE uint32_t pf_desc_mn(uint32_t saddr) { return saddr >> 4; }
+MF_DEVICE uint32_t pf_desc_k(uint32_t saddr) { return saddr >> 4 | ((uint32_t)(PF_HALF >> 4) << 16); }
+
+// D (TMEM) (+)= A * B with B from shared memory and A from shared memory or TMEM; lower words of the descriptors.
+MF_DEVICE void pf_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %5};\n\t"
+        "mov.b64 b, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(PF_DESC_HI)
+        : "memory");
+}
+MF_DEVICE void pf_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+        "mov.b64 b, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(PF_DESC_HI)
+        : "memory");
+}
+// One thread of the warp, known to the compiler as one: what it computes stays in uniform registers.
+MF_DEVICE bool pf_elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 
 // One box of the pages' map (d, row of the page, head, page, tensor).
@@ -78,6 +102,54 @@ MF_DEVICE void tma_load_page(void* dst, const CUtensorMap* tm, uint64_t* bar, in
         : "memory");
 }
 
+// Two floats as one 64-bit operand of the packed fp32 instructions.
+typedef unsigned long long f32x2;
+MF_DEVICE f32x2 pf_two(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+MF_DEVICE float2 pf_each(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+MF_DEVICE f32x2 pf_fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+MF_DEVICE f32x2 pf_add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+MF_DEVICE float pf_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^y of two finite y on the FMA units: y = n + r, |r| <= 1/2, a polynomial of
+// degree 5 for 2^r (minimax, relative error 2^-23.6), n added to its exponent.
+// Below 2^-126 the result is a tiny number instead of zero.
+MF_DEVICE float2 pf_exp2_fma(f32x2 y) {
+    const float2 c = pf_each(y);
+    y = pf_two(fmaxf(c.x, -126.f), fmaxf(c.y, -126.f));
+    const f32x2 magic = pf_two(12582912.f, 12582912.f);  // 1.5 * 2^23: the low bits of the sum are n
+    const f32x2 t = pf_add2(y, magic);
+    const f32x2 n = pf_add2(t, pf_two(-12582912.f, -12582912.f));
+    const f32x2 r = pf_fma2(n, pf_two(-1.f, -1.f), y);
+    f32x2 q = pf_two(1.3276472e-3f, 1.3276472e-3f);
+    q = pf_fma2(q, r, pf_two(9.675541e-3f, 9.675541e-3f));
+    q = pf_fma2(q, r, pf_two(5.5507131e-2f, 5.5507131e-2f));
+    q = pf_fma2(q, r, pf_two(2.402212e-1f, 2.402212e-1f));
+    q = pf_fma2(q, r, pf_two(6.9314694e-1f, 6.9314694e-1f));
+    q = pf_fma2(q, r, pf_two(1.0000001f, 1.0000001f));
+    const float2 ti = pf_each(t), qi = pf_each(q);
+    return make_float2(__int_as_float(__float_as_int(qi.x) + (__float_as_int(ti.x) << 23)),
+                       __int_as_float(__float_as_int(qi.y) + (__float_as_int(ti.y) << 23)));
+}
+
 template <typename T> MF_DEVICE uint32_t pf_pack(float a, float b);
 template <> MF_DEVICE uint32_t pf_pack<__nv_bfloat16>(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -86,6 +158,23 @@ template <> MF_DEVICE uint32_t pf_pack<__nv_bfloat16>(float a, float b) {
 template <> MF_DEVICE uint32_t pf_pack<__half>(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 16 columns of this warp's lanes
+MF_DEVICE void pf_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    tmem_wait_ld();
+}
+MF_DEVICE void pf_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
 }
 
 // The row tile `tile` of the batch: sequences of more than min_rows rows, in
@@ -132,7 +221,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     uint8_t* vs = smem + PF_STAGES * TILE;
     uint8_t* qs = vs + PF_STAGES * TILE;
     __shared__ __align__(8) uint64_t k_full[PF_STAGES], k_free[PF_STAGES], v_full[PF_STAGES], v_free[PF_STAGES];
-    __shared__ __align__(8) uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
+    __shared__ __align__(8) uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], drain;
     __shared__ uint32_t tmem_base_s;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -146,7 +235,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 128);
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 128);
+            mbar_init(&p_full[i][0], 128);
+            mbar_init(&p_full[i][1], 128);
             mbar_init(&o_full[i], 1);
         }
         mbar_init(&drain, 1);
@@ -181,7 +271,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     bool failed = false;
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 9 || warp == 10) {
             const bool is_k = warp == 9;
             const CUtensorMap* tm = is_k ? &tk : &tv;
@@ -238,25 +328,27 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                 const unsigned long long d2 = globaltimer_ns() + a.timeout_ns;
                 for (int j = max(0, issued - PF_STAGES); j < issued; ++j) mbar_wait(&full[j % PF_STAGES], (uint32_t)(j / PF_STAGES) & 1u, d2, f2);
             }
-        } else if (warp == 8 && lane == 0 && nt > 0) {
+        } else if (warp == 8 && nt > 0 && pf_elect()) {
             constexpr uint32_t idesc_s = fa_idesc(128, PF_KT, BF);
             constexpr uint32_t idesc_o = fa_idesc(128, D, BF) | (1u << 16);  // B's rows run along K
             bool any = false;
+            const uint32_t k_lo = pf_desc_mn(smem_u32(ks)), q_lo = pf_desc_mn(smem_u32(qs)), v_lo = pf_desc_k(smem_u32(vs));
             auto issue_s = [&](int i, int j) {  // S_i = Q_i K_j^T
-                const uint32_t kb = smem_u32(ks + (j % PF_STAGES) * TILE), qb = smem_u32(qs + i * TILE);
+                const uint32_t kb = k_lo + (uint32_t)(j % PF_STAGES) * (TILE >> 4), qb = q_lo + (uint32_t)i * (TILE >> 4);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (uint32_t)(k >> 2) * PF_HALF + (uint32_t)(k & 3) * 32;
-                    umma_bf16(tmem + 128u * i, sw128_kmajor_desc(qb + off), sw128_kmajor_desc(kb + off), idesc_s, k > 0 ? 1u : 0u);
+                    const uint32_t off = ((uint32_t)(k >> 2) * PF_HALF + (uint32_t)(k & 3) * 32) >> 4;
+                    pf_mma_ss(tmem + 128u * i, qb + off, kb + off, idesc_s, k > 0 ? 1u : 0u);
                 }
                 umma_commit(&s_full[i]);
                 any = true;
             };
-            auto issue_o = [&](int i, int j) {  // O_i += P_i V_j
-                const uint32_t vb = smem_u32(vs + (j % PF_STAGES) * TILE);
+            auto issue_o = [&](int i, int j, int half) {  // O_i += P_i V_j, 64 keys
+                const uint32_t vb = v_lo + (uint32_t)(j % PF_STAGES) * (TILE >> 4) + half * (PF_KT / 2 * 128 >> 4);
+                const uint32_t pb = tmem + 128u * i + 32u * half;
 #pragma unroll
-                for (int k = 0; k < PF_KT / 16; ++k)
-                    umma_ts(tmem + 256u + 128u * i, tmem + 128u * i + 8u * k, pf_desc_rows_k(vb + 2048u * k), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+                for (int k = 0; k < PF_KT / 32; ++k)
+                    pf_mma_ts(tmem + 256u + 128u * i, pb + 8u * k, vb + (2048u * k >> 4), idesc_o, (j > 0 || half > 0 || k > 0) ? 1u : 0u);
             };
             for (int i = 0; i < (two ? 2 : 1); ++i) mbar_wait(&q_full[i], 0, deadline, failed);
             mbar_wait(&k_full[0], 0, deadline, failed);
@@ -270,9 +362,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                 const bool more = j + 1 < nt;
                 mbar_wait(&v_full[j % PF_STAGES], (uint32_t)(j / PF_STAGES) & 1u, deadline, failed);
                 for (int i = 0; i < (two ? 2 : 1); ++i) {
-                    if (!mbar_wait(&p_full[i], (uint32_t)j & 1u, deadline, failed)) break;
+                    if (!mbar_wait(&p_full[i][0], (uint32_t)j & 1u, deadline, failed)) break;
                     tc_fence_after();
-                    issue_o(i, j);
+                    issue_o(i, j, 0);
+                    if (!mbar_wait(&p_full[i][1], (uint32_t)j & 1u, deadline, failed)) break;
+                    tc_fence_after();
+                    issue_o(i, j, 1);
                     if (more) {
                         if (i == 0 && !mbar_wait(&k_full[(j + 1) % PF_STAGES], (uint32_t)((j + 1) / PF_STAGES) & 1u, deadline, failed)) break;
                         tc_fence_after();
@@ -293,7 +388,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int i = warp >> 2;  // row tile
         const int r = threadIdx.x & 127;
         const int row = pt.r0 + 128 * i + r;  // of the sequence
@@ -334,50 +429,77 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) tmem_ld32_nowait(trow + 128u * i + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(sr + 32 * q));
                 tmem_wait_ld();
-                float sv[128];
-                if (k0 + PF_KT - 1 <= hi_all && k0 >= lo_all && ok == 0xffffu) {
-#pragma unroll
-                    for (int c = 0; c < 128; ++c) sv[c] = __uint_as_float(sr[c]);
-                } else {
+                const bool plain = k0 + PF_KT - 1 <= hi_all && k0 >= lo_all && ok == 0xffffu;
+                if (!plain) {
 #pragma unroll
                     for (int c = 0; c < 128; ++c)
-                        sv[c] = k0 + c <= my_pos && k0 + c >= my_lo && (ok >> (c >> 3) & 1) ? __uint_as_float(sr[c]) : -INFINITY;
+                        if (!(k0 + c <= my_pos && k0 + c >= my_lo && (ok >> (c >> 3) & 1))) sr[c] = 0xff800000u;  // -inf
                 }
-                float m4[4] = {sv[0], sv[1], sv[2], sv[3]};
+                float m4[4];
 #pragma unroll
-                for (int c = 4; c < 128; ++c) m4[c & 3] = fmaxf(m4[c & 3], sv[c]);
-                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c2;
+                for (int c = 0; c < 4; ++c) m4[c] = __uint_as_float(sr[c]);
+#pragma unroll
+                for (int c = 4; c < 124; c += 8)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) m4[u] = pf_max3(m4[u], __uint_as_float(sr[c + u]), __uint_as_float(sr[c + 4 + u]));
+#pragma unroll
+                for (int u = 0; u < 4; ++u) m4[u] = fmaxf(m4[u], __uint_as_float(sr[124 + u]));
+                const float mx = fmaxf(pf_max3(m4[0], m4[1], m4[2]), m4[3]) * c2;
                 const bool bump = mx > m + 8.f;  // also the first keys of a row (m = -inf)
                 const float mu = bump ? mx : m;
                 const float base = mu == -INFINITY ? 0.f : mu;
                 const float alpha = bump ? ex2_approx(m - base) : 1.f;
-                float s4[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t pk[64];
-#pragma unroll
-                for (int c = 0; c < 128; c += 2) {
-                    const float e0 = ex2_approx(fmaf(sv[c], c2, -base)), e1 = ex2_approx(fmaf(sv[c + 1], c2, -base));
-                    s4[c & 2] += e0;
-                    s4[(c & 2) + 1] += e1;
-                    pk[c >> 1] = pf_pack<T>(e0, e1);
-                }
-                l = fmaf(l, alpha, (s4[0] + s4[1]) + (s4[2] + s4[3]));
                 m = mu;
-                tmem_st32(trow + 128u * i, *reinterpret_cast<uint32_t(*)[32]>(pk));
-                tmem_st32(trow + 128u * i + 32, *reinterpret_cast<uint32_t(*)[32]>(pk + 32));
                 // O_i holds the tiles before j (S_i was issued after them): rescale where the maximum moved
                 if (j > 0 && __any_sync(0xffffffffu, bump)) {
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(trow + 256u + 128u * i + c, o);
+                    for (int c = 0; c < D; c += 16) {
+                        uint32_t o[16];
+                        pf_ld16(trow + 256u + 128u * i + c, o);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        tmem_st32(trow + 256u + 128u * i + c, o);
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        pf_st16(trow + 256u + 128u * i + c, o);
                     }
                 }
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(&p_full[i]);
+                // P in two halves of 64 keys: the tensor core starts on the first while the second is made. One pair of
+                // every four takes its exponentials on the FMA units, since the special-function unit alone would need
+                // as long as the tensor core for the whole tile.
+                const f32x2 c2c2 = pf_two(c2, c2), bb = pf_two(-base, -base);
+                f32x2 s2[2] = {pf_two(0.f, 0.f), pf_two(0.f, 0.f)};
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t pk[32];
+                    if (plain) {
+#pragma unroll
+                        for (int c = 0; c < 64; c += 2) {
+                            const f32x2 y = pf_fma2(pf_two(__uint_as_float(sr[64 * half + c]), __uint_as_float(sr[64 * half + c + 1])), c2c2, bb);
+                            float2 e;
+                            if ((c & 6) == 6) {
+                                e = pf_exp2_fma(y);
+                            } else {
+                                e = pf_each(y);
+                                e.x = ex2_approx(e.x);
+                                e.y = ex2_approx(e.y);
+                            }
+                            s2[c >> 1 & 1] = pf_add2(s2[c >> 1 & 1], pf_two(e.x, e.y));
+                            pk[c >> 1] = pf_pack<T>(e.x, e.y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 64; c += 2) {
+                            const float e0 = ex2_approx(fmaf(__uint_as_float(sr[64 * half + c]), c2, -base));
+                            const float e1 = ex2_approx(fmaf(__uint_as_float(sr[64 * half + c + 1]), c2, -base));
+                            s2[c >> 1 & 1] = pf_add2(s2[c >> 1 & 1], pf_two(e0, e1));
+                            pk[c >> 1] = pf_pack<T>(e0, e1);
+                        }
+                    }
+                    tmem_st32(trow + 128u * i + 32 * half, pk);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&p_full[i][half]);
+                }
+                const float2 sum = pf_each(pf_add2(s2[0], s2[1]));
+                l = fmaf(l, alpha, sum.x + sum.y);
             }
             if (nt > 0) mbar_wait(&o_full[i], 0, deadline, failed);
             tc_fence_after();
