@@ -191,7 +191,7 @@ struct FewPlan {
     int threads, RT;
 };
 template <int D, int RT> FewPlan simt_plan() {
-    return {(const void*)&mf::paged_simt_kernel<float, D, RT>, (const void*)&mf::paged_join_kernel<float, D, RT, mf::PA_SIMT_KT>,
+    return {(const void*)&mf::paged_simt_kernel<D, RT>, (const void*)&mf::paged_join_kernel<float, D, RT, mf::PA_SIMT_KT>,
             (size_t)mf::paged_simt_smem<RT, D>(), mf::PA_SIMT_THREADS, RT};
 }
 template <typename T, int D, int MT> FewPlan mma_plan() {
@@ -230,7 +230,7 @@ int resident(const void* fn, int threads, size_t smem, int* blocks) {
 }
 
 // Blocks per SM that the workspace of the kernels for few rows is sized for.
-int per_sm(int RT) { return RT == 16 ? 4 : RT == 32 ? 2 : 1; }
+int per_sm(int RT) { return RT == 16 ? 4 : 2; }
 
 // Shares of the keys in which the chunk kernel works when its row tiles alone
 // leave SMs idle (1: none).
@@ -246,10 +246,6 @@ const void* fa_fn(int dtype, int d, bool join) {
     return dtype == MF_F16 ? (d == 64 ? fa_fn2<__half, 64>(join) : fa_fn2<__half, 128>(join))
                            : (d == 64 ? fa_fn2<__nv_bfloat16, 64>(join) : fa_fn2<__nv_bfloat16, 128>(join));
 }
-
-// Sequences of more query rows (new tokens x heads of a group) than this go to
-// the chunk kernel, which works on 256 rows at a time.
-constexpr int FEW_ROWS = 32;
 
 size_t part_bytes(int blocks, int RT, int d) { return (size_t)2 * blocks * RT * (d + 2) * sizeof(float); }
 
@@ -339,9 +335,9 @@ int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* d, voi
 
 size_t mf_paged_attention_workspace_bytes(int n_tokens, int n_heads, int n_kv_heads, int d_head, int dtype) {
     if (n_tokens <= 0 || n_heads <= 0 || n_kv_heads <= 0 || (d_head != 64 && d_head != 128) || !known_dtype(dtype)) return 0;
-    const size_t few = part_bytes(num_sms(), 64, d_head);  // the same for 2 blocks per SM of 32 rows and 4 of 16
+    const size_t few = part_bytes(num_sms(), 64, d_head);  // 4 blocks per SM of 16 rows, 2 of 32
     const size_t split = (size_t)chunk_split(n_tokens, n_heads, n_kv_heads) * n_tokens * n_heads * (d_head + 2) * sizeof(float);
-    return few + (dtype == MF_F32 ? 0 : split);
+    return few + (dtype == MF_F32 ? part_bytes(2 * num_sms(), 64, d_head) : split);
 }
 
 int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void* stream) {
@@ -373,7 +369,6 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
     a.n_heads = d->n_heads;
     a.G = G;
     a.window = d->window;
-    a.part = (float*)d->workspace;
     const int most = std::min(d->max_new > 0 ? d->max_new : d->n_tokens, d->n_tokens);
     cudaStream_t st = mf::resolve_stream(stream);
 
@@ -381,27 +376,53 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
     if (!a.status) return fail(MF_E_CUDA, "status symbol");
     a.timeout_ns = timeout_ns();
 
-    // 16-bit pages: sequences of more than FEW_ROWS rows go to the tensor-core
-    // chunk kernel. A batch of one sequence is served by one kernel alone.
-    const bool chunks = kv->dtype != MF_F32 && (long long)most * G > FEW_ROWS;
+    // Sequences of more than few_rows query rows (new tokens x heads of a group)
+    // go to the chunk kernels, which work on 256 (16-bit pages, tensor cores) or
+    // 64 rows at a time (fp32), the others to the kernels for few rows. A batch
+    // of one sequence is served by one of them alone.
+    const bool f32 = kv->dtype == MF_F32;
+    const int few_rows = f32 ? 16 : 32;
+    const bool chunks = (long long)most * G > few_rows;
     const bool few = !chunks || kv->n_seqs > 1;
     cudaError_t e = cudaSuccess;
     CUtensorMap tk, tv;
     int run = page_run(p.page_size), at = 0;
-    if (kv->dtype != MF_F32) {
+    if (!f32) {
         rc = page_tmaps(&tk, &tv, p, D, kv->dtype, run, &at);
         if (rc) return rc;
     }
-    if (chunks) {
+    // parts of the kernels for few rows, of the fp32 chunk kernel, of the split chunk kernel
+    float* part_few = (float*)d->workspace;
+    float* part_chunk = part_few + part_bytes(num_sms(), 64, D) / sizeof(float);
+    auto share_out = [&](const FewPlan& s, int min_rows, int max_rows, float* part) {  // a kernel of paged_work.cuh and its join
+        a.min_rows = min_rows;
+        a.max_rows = max_rows;
+        a.part = part;
+        int blocks = 0;
+        const int r = resident(s.kernel, s.threads, s.smem, &blocks);
+        if (r) return r;
+        blocks = std::min(blocks, per_sm(s.RT) * num_sms());
+        void* f32_args[] = {&p, &a};
+        void* args[] = {&tk, &tv, &p, &a, &run, &at};
+        e = launch(s.kernel, dim3(blocks), dim3(s.threads), s.smem, st, f32 ? f32_args : args);
+        if (e == cudaSuccess && blocks > 1) {
+            void* jargs[] = {&p, &a, &blocks};
+            e = launch(s.join, dim3(blocks - 1), dim3(256), 0, st, jargs);
+        }
+        return e == cudaSuccess ? MF_OK : fail(MF_E_CUDA, cudaGetErrorString(e));
+    };
+    if (chunks && f32) {
+        rc = share_out(few_plan(kv->dtype, D, 64), few ? few_rows : 0, 0x7fffffff, part_chunk);
+        if (rc) return rc;
+    } else if (chunks) {
         mf::PagedFa f = {};
         f.run = run;
         f.at = at;
-        f.min_rows = few ? FEW_ROWS : 0;
-        a.max_rows = few ? FEW_ROWS : 0;
+        f.min_rows = few ? few_rows : 0;
         f.n_split = chunk_split(d->n_tokens, d->n_heads, kv->n_kv_heads);
         if (d->max_len > 0) f.n_split = std::min(f.n_split, std::max(1, d->max_len / (4 * mf::PF_KT)));
         const size_t rows = (size_t)d->n_tokens * d->n_heads;
-        f.part_o = a.part + (mf_paged_attention_workspace_bytes(d->n_tokens, d->n_heads, kv->n_kv_heads, D, MF_F32) + 3) / 4;
+        f.part_o = part_chunk;
         f.part_ml = (float2*)(f.part_o + f.n_split * rows * D);
         const void* fn = fa_fn(kv->dtype, D, false);
         const size_t smem = D == 64 ? mf::pf_smem<64>() : mf::pf_smem<128>();
@@ -418,26 +439,11 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
             void* jargs[] = {&p, &a, &f};
             e = launch(fa_fn(kv->dtype, D, true), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, jargs);
         }
+        if (e != cudaSuccess) return fail(MF_E_CUDA, cudaGetErrorString(e));
     }
-    if (few && e == cudaSuccess) {
-        const FewPlan s = few_plan(kv->dtype, D, chunks ? std::min<long long>(FEW_ROWS, (long long)most * G) : (long long)most * G);
-        int blocks = 0;
-        rc = resident(s.kernel, s.threads, s.smem, &blocks);
-        if (rc) return rc;
-        blocks = std::min(blocks, per_sm(s.RT) * num_sms());
-        if (kv->dtype == MF_F32) {
-            void* args[] = {&p, &a};
-            e = launch(s.kernel, dim3(blocks), dim3(s.threads), s.smem, st, args);
-        } else {
-            void* args[] = {&tk, &tv, &p, &a, &run, &at};
-            e = launch(s.kernel, dim3(blocks), dim3(s.threads), s.smem, st, args);
-        }
-        if (e == cudaSuccess && blocks > 1) {
-            void* jargs[] = {&p, &a, &blocks};
-            e = launch(s.join, dim3(blocks - 1), dim3(256), 0, st, jargs);
-        }
-    }
-    return e == cudaSuccess ? MF_OK : fail(MF_E_CUDA, cudaGetErrorString(e));
+    return few ? share_out(few_plan(kv->dtype, D, std::min<long long>((long long)most * G, chunks ? few_rows : 0x7fffffff)), 0,
+                           chunks ? few_rows : 0x7fffffff, part_few)
+               : MF_OK;
 }
 
 int mf_paged_status(int* status, int clear) {

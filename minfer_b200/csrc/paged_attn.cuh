@@ -12,6 +12,9 @@
 //   RT = 16 rows (a few tokens): four groups of 64 threads share D for S and
 //   the keys for P V, so that a thread's tile stays 4 x 4 and shared memory
 //   is not what bounds it; their sums are added at the end of an item.
+// Tiles are stored without padding, 16-byte pieces c of row r at c ^ (r & 7)
+// (no bank conflicts in either direction), so that two CTAs fit an SM and one
+// computes while the other's softmax waits at a barrier.
 #pragma once
 
 #include "paged_work.cuh"
@@ -21,69 +24,66 @@ namespace mf {
 constexpr int PA_SIMT_KT = 64;
 constexpr int PA_SIMT_THREADS = 256;
 
+// Q, K, V, the partial scores, and alpha per row
 template <int RT, int D> constexpr int paged_simt_smem() {
-    // Q, K, V (padded rows), S partials, alpha and l per row
-    return (RT * (D + 4) + 2 * PA_SIMT_KT * (D + 4) + (64 / RT) * RT * (PA_SIMT_KT + 4) + 2 * RT) * 4 + PA_SIMT_KT * 4;
+    return (RT * D + 2 * PA_SIMT_KT * D + 64 * PA_SIMT_KT + RT) * 4;
 }
 
-// D-element rows [k0, k0 + 64) of one head of sequence b into shared memory as
-// fp32; rows outside [lo, hi) or without a page become zeros. `valid` (with K) notes which rows hold keys.
-template <typename T, int D>
-MF_DEVICE void paged_simt_load(float* dst, const T* base, const PagedKv& p, int b, int h, int k0, int lo, int hi, int* valid) {
+// Element c of row r of a tile whose rows have W elements.
+template <int W> MF_DEVICE int pa_at(int r, int c) { return r * W + (((c >> 2) ^ (r & 7)) << 2) + (c & 3); }
+
+// Rows [k0, k0 + 64) of one head of sequence b into shared memory; rows outside
+// [lo, hi) or without a page become zeros. Returns which rows have a page (the same in every thread).
+template <int D>
+MF_DEVICE unsigned long long paged_simt_load(float* dst, const float* base, const PagedKv& p, int b, int h, int k0, int lo, int hi) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr int V = D / 32;
-#pragma unroll 4
-    for (int i = warp; i < PA_SIMT_KT; i += PA_SIMT_THREADS / 32) {
-        const int key = k0 + i;
-        const int page = key >= lo && key < hi ? paged_page(p, b, key) : -1;
-        if (valid && lane == 0) valid[i] = page >= 0;
-        float* d = dst + i * (D + 4) + lane * V;
-        const T* src = base + (page >= 0 ? page * p.page_stride + (long long)h * p.head_stride + (key % p.page_size) * p.row_stride + lane * V : 0);
-        if constexpr (sizeof(T) == 4) {
-            const uint32_t s = (uint32_t)__cvta_generic_to_shared(d);
-            if constexpr (V == 4) {
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(src), "r"(page >= 0 ? 16 : 0) : "memory");
-            } else {
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(s), "l"(src), "r"(page >= 0 ? 8 : 0) : "memory");
-            }
-        } else {
-            PackV<T, V> x = {};
-            if (page >= 0) x = *reinterpret_cast<const PackV<T, V>*>(src);
+    constexpr int C = D / 4, RPI = 32 / C;  // pieces of a row, rows per access of a warp
+    // each lane looks up two rows of the tile, and the warp shares them
+    long long off[2];
+    unsigned have[2];
 #pragma unroll
-            for (int e = 0; e < V; ++e) d[e] = to_f<T>(x.e[e]);
-        }
+    for (int u = 0; u < 2; ++u) {
+        const int key = k0 + 32 * u + lane;
+        const int page = key >= lo && key < hi ? paged_page(p, b, key) : -1;
+        off[u] = page < 0 ? -1 : page * p.page_stride + (long long)h * p.head_stride + (long long)(key % p.page_size) * p.row_stride;
+        have[u] = __ballot_sync(0xffffffffu, page >= 0);
+    }
+#pragma unroll
+    for (int i = 0; i < PA_SIMT_KT / 8 / RPI; ++i) {
+        const int row = (i * 8 + warp) * RPI + lane / C, c = lane % C * 4;
+        const long long o0 = __shfl_sync(0xffffffffu, off[0], row & 31), o1 = __shfl_sync(0xffffffffu, off[1], row & 31);
+        const long long o = row < 32 ? o0 : o1;
+        const uint32_t s = (uint32_t)__cvta_generic_to_shared(dst + pa_at<D>(row, c));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(base + (o < 0 ? 0 : o + c)), "r"(o < 0 ? 0 : 16) : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
+    return (unsigned long long)have[1] << 32 | have[0];
 }
 
-template <typename T, int D, int RT>
-__global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const PagedKv p, const PagedAttn a) {
-    constexpr int KT = PA_SIMT_KT, NG = 64 / RT, GT = PA_SIMT_THREADS / NG, LD = D + 4, LS = KT + 4;
+template <int D, int RT>
+__global__ void __launch_bounds__(PA_SIMT_THREADS, 2) paged_simt_kernel(const PagedKv p, const PagedAttn a) {
+    constexpr int KT = PA_SIMT_KT, NG = 64 / RT, GT = PA_SIMT_THREADS / NG;
     constexpr int NC = D / 64;            // float4 columns of O per thread
     constexpr int TPR = PA_SIMT_THREADS / RT, KPT = KT / TPR;  // softmax: threads per row, keys per thread
     extern __shared__ __align__(16) float paged_smem[];
     float* Qs = paged_smem;
-    float* Ks = Qs + RT * LD;
-    float* Vs = Ks + KT * LD;
-    float* Ss = Vs + KT * LD;
-    float* alpha_s = Ss + NG * RT * LS;
-    float* l_s = alpha_s + RT;
-    int* valid = reinterpret_cast<int*>(l_s + RT);
-    __shared__ long long sh[34];
+    float* Ks = Qs + RT * D;
+    float* Vs = Ks + KT * D;
+    float* Ss = Vs + KT * D;             // [NG][RT][KT]
+    float* alpha_s = Ss + NG * RT * KT;  // [RT]
     pdl_wait();
     pdl_launch_dependents();  // after the wait: see paged_join_kernel
 
     PagedItem it;
     long long share;
-    const long long total = paged_find<RT, KT>(p, a, blockIdx.x, gridDim.x, sh, share, it);
+    const long long total = paged_find<RT, KT>(p, a, blockIdx.x, gridDim.x, reinterpret_cast<long long*>(Ks), share, it);
     const long long w0 = blockIdx.x * share, w1 = min(w0 + share, total);
     if (w0 >= w1) return;
-
     const int tid = threadIdx.x, grp = tid / GT, tg = tid % GT;
     const int ty = tg / 16, tx = tg % 16;  // rows 4 ty .., keys tx + 16 j, columns 4 tx + 64 j
     const int srow = tid / TPR, sk = tid % TPR;
-    const T* kb = reinterpret_cast<const T*>(p.k);
-    const T* vb = reinterpret_cast<const T*>(p.v);
+    const float* kb = reinterpret_cast<const float*>(p.k);
+    const float* vb = reinterpret_cast<const float*>(p.v);
 
     for (long long w = w0; w < w1;) {
         const int j0 = (int)max(w - it.start, 0ll), j1 = (int)min((long long)it.tiles, w1 - it.start);
@@ -91,12 +91,13 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
         const int rows = min(RT, it.s.n * a.G - it.r0);
         const int kt0 = it.k.lo / KT;
         __syncthreads();
-        paged_simt_load<T, D>(Ks, kb, p, it.b, it.h, (kt0 + j0) * KT, it.k.lo, it.k.hi, valid);
-        for (int i = tid; i < RT * D; i += PA_SIMT_THREADS) {
-            const int r = i / D, row = it.r0 + r;
-            Qs[r * LD + i % D] = r < rows ? to_f<T>(reinterpret_cast<const T*>(a.q)[(long long)(it.s.row + row / a.G) * a.q_stride +
-                                                                                   (long long)(it.h * a.G + row % a.G) * D + i % D]) * a.scale2
-                                          : 0.f;
+        unsigned long long pages = paged_simt_load<D>(Ks, kb, p, it.b, it.h, (kt0 + j0) * KT, it.k.lo, it.k.hi);
+        for (int i = tid; i < RT * D / 4; i += PA_SIMT_THREADS) {
+            const int r = i / (D / 4), c = i % (D / 4) * 4, row = it.r0 + r;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows) v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + (long long)(it.s.row + row / a.G) * a.q_stride +
+                                                                 (long long)(it.h * a.G + row % a.G) * D + c);
+            *reinterpret_cast<float4*>(Qs + pa_at<D>(r, c)) = make_float4(v.x * a.scale2, v.y * a.scale2, v.z * a.scale2, v.w * a.scale2);
         }
         float o[4][4 * NC];
 #pragma unroll
@@ -109,7 +110,8 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
 
         for (int j = j0; j < j1; ++j) {
             const int k0 = (kt0 + j) * KT;
-            paged_simt_load<T, D>(Vs, vb, p, it.b, it.h, k0, it.k.lo, it.k.hi, nullptr);
+            const unsigned long long have = pages;
+            paged_simt_load<D>(Vs, vb, p, it.b, it.h, k0, it.k.lo, it.k.hi);
             asm volatile("cp.async.wait_group 1;" ::: "memory");
             __syncthreads();  // K (and Q) are there
             float acc[4][4] = {};
@@ -117,9 +119,9 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
             for (int d = grp * (D / NG); d < (grp + 1) * (D / NG); d += 4) {
                 float4 qv[4], kv[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(Qs + (4 * ty + i) * LD + d);
+                for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(Qs + pa_at<D>(4 * ty + i, d));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) kv[i] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * i) * LD + d);
+                for (int i = 0; i < 4; ++i) kv[i] = *reinterpret_cast<const float4*>(Ks + pa_at<D>(tx + 16 * i, d));
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) Ss[(grp * RT + 4 * ty + i) * LS + tx + 16 * k] = acc[i][k];
+                for (int k = 0; k < 4; ++k) Ss[pa_at<KT>(grp * RT + 4 * ty + i, tx + 16 * k)] = acc[i][k];
             __syncthreads();
             // softmax of row srow over its KPT keys sk, sk + TPR, ...
             float sv[KPT], mx = m;
@@ -142,8 +144,8 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
                 const int kk = sk + TPR * k, key = k0 + kk;
                 float x = 0.f;
 #pragma unroll
-                for (int g = 0; g < NG; ++g) x += Ss[(g * RT + srow) * LS + kk];
-                sv[k] = key <= my_pos && key >= my_lo && valid[kk] ? x : -INFINITY;
+                for (int g = 0; g < NG; ++g) x += Ss[pa_at<KT>(g * RT + srow, kk)];
+                sv[k] = key <= my_pos && key >= my_lo && (have >> kk & 1) ? x : -INFINITY;
                 mx = fmaxf(mx, sv[k]);
             }
 #pragma unroll
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
             for (int k = 0; k < KPT; ++k) {
                 const float e = exp2f(sv[k] - base);
                 sum += e;
-                Ss[srow * LS + sk + TPR * k] = e;  // group 0's plane: only this thread reads or writes the entry
+                Ss[pa_at<KT>(srow, sk + TPR * k)] = e;  // group 0's plane: only this thread reads or writes the entry
             }
 #pragma unroll
             for (int off = TPR / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
@@ -164,7 +166,7 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
             if (sk == 0) alpha_s[srow] = al;
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncthreads();  // P, alpha and V are there; K is free
-            if (j + 1 < j1) paged_simt_load<T, D>(Ks, kb, p, it.b, it.h, k0 + KT, it.k.lo, it.k.hi, valid);
+            if (j + 1 < j1) pages = paged_simt_load<D>(Ks, kb, p, it.b, it.h, k0 + KT, it.k.lo, it.k.hi);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float al4 = alpha_s[4 * ty + i];
@@ -175,12 +177,12 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
             for (int k = grp * (KT / NG); k < (grp + 1) * (KT / NG); k += 4) {
                 float4 pv[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4*>(Ss + (4 * ty + i) * LS + k);
+                for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4*>(Ss + pa_at<KT>(4 * ty + i, k));
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
                     for (int n = 0; n < NC; ++n) {
-                        const float4 v = *reinterpret_cast<const float4*>(Vs + (k + kk) * LD + 4 * tx + 64 * n);
+                        const float4 v = *reinterpret_cast<const float4*>(Vs + pa_at<D>(k + kk, 4 * tx + 64 * n));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float pr = reinterpret_cast<const float*>(&pv[i])[kk];
@@ -193,9 +195,9 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
             }
             __syncthreads();  // V and P are free
         }
-        // the groups' sums of O, in order, in the K tile's place
+        // the groups' sums of O, in order, in the K tile's place; m and l per row in the scores'
         if constexpr (NG > 1) {
-            float* Os = Ks;  // [NG][RT][D] <= 2 * KT * LD
+            float* Os = Ks;  // [NG][RT][D] <= KT * D
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -203,9 +205,11 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
                     *reinterpret_cast<float4*>(Os + (grp * RT + 4 * ty + i) * D + 4 * tx + 64 * n) =
                         make_float4(o[i][4 * n], o[i][4 * n + 1], o[i][4 * n + 2], o[i][4 * n + 3]);
         }
+        float* l_s = Ss;
+        float* m_s = Ss + RT;
         if (sk == 0) {
             l_s[srow] = l;
-            alpha_s[srow] = m;
+            m_s[srow] = m;
         }
         __syncthreads();
         const bool whole = j0 == 0 && j1 == it.tiles;
@@ -217,17 +221,12 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS) paged_simt_kernel(const Paged
             if (whole) {
                 const float inv = l_s[r] == 0.f ? 0.f : 1.0f / l_s[r];
                 const int row = it.r0 + r;
-                PackV<T, 4> y;
-                y.e[0] = from_f<T>(v.x * inv);
-                y.e[1] = from_f<T>(v.y * inv);
-                y.e[2] = from_f<T>(v.z * inv);
-                y.e[3] = from_f<T>(v.w * inv);
-                *reinterpret_cast<PackV<T, 4>*>(reinterpret_cast<T*>(a.out) + (long long)(it.s.row + row / a.G) * a.out_stride +
-                                                (long long)(it.h * a.G + row % a.G) * D + c) = y;
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + (long long)(it.s.row + row / a.G) * a.out_stride +
+                                           (long long)(it.h * a.G + row % a.G) * D + c) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
             } else {
                 *reinterpret_cast<float4*>(part + r * D + c) = v;
                 if (c == 0) {
-                    ml[2 * r] = alpha_s[r];
+                    ml[2 * r] = m_s[r];
                     ml[2 * r + 1] = l_s[r];
                 }
             }

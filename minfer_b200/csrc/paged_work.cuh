@@ -26,7 +26,7 @@ struct PagedAttn {
     long long q_stride;
     float scale2;  // softmax scale * log2(e)
     int n_heads, G, window;
-    int max_rows;  // sequences of more rows (n_b * G) are another kernel's (0: none are)
+    int min_rows, max_rows;  // sequences of other numbers of rows (n_b * G) are another kernel's: min_rows < rows <= max_rows
     float* part;   // (O, m, l) of divided items: [2 * grid][RT][D], then [2 * grid][RT][2]
     int* status;   // bit 2: a wait gave up
     unsigned long long timeout_ns;
@@ -49,7 +49,7 @@ template <int KT> MF_DEVICE int paged_tiles(const PagedSpan& k) { return max((k.
 // Tiles of one KV head of sequence b (0: no rows, or another kernel's)
 template <int RT, int KT> MF_DEVICE int paged_head_work(const PagedSeq& s, const PagedAttn& a) {
     const int rows = s.n * a.G;
-    if (rows == 0 || (a.max_rows > 0 && rows > a.max_rows)) return 0;
+    if (rows <= a.min_rows || rows > a.max_rows) return 0;
     int w = 0;
     for (int r = 0; r < rows; r += RT) w += 1 + paged_tiles<KT>(paged_span(s, a, r, RT));
     return w;
@@ -156,7 +156,7 @@ template <int RT, int KT> MF_DEVICE void paged_next(const PagedKv& p, const Page
             it.h = 0;
             do {
                 it.s = paged_seq(p, ++it.b);
-            } while (it.s.n == 0 || (a.max_rows > 0 && it.s.n * a.G > a.max_rows));
+            } while (it.s.n * a.G <= a.min_rows || it.s.n * a.G > a.max_rows);
         }
     }
     it.k = paged_span(it.s, a, it.r0, RT);
