@@ -394,34 +394,45 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
     // parts of the kernels for few rows, of the fp32 chunk kernel, of the split chunk kernel
     float* part_few = (float*)d->workspace;
     float* part_chunk = part_few + part_bytes(num_sms(), 64, D) / sizeof(float);
-    auto share_out = [&](const FewPlan& s, int min_rows, int max_rows, float* part) {  // a kernel of paged_work.cuh and its join
-        a.min_rows = min_rows;
-        a.max_rows = max_rows;
-        a.part = part;
-        int blocks = 0;
-        const int r = resident(s.kernel, s.threads, s.smem, &blocks);
+    // a kernel of paged_work.cuh, and the one that joins its parts
+    struct Shared {
+        FewPlan s;
+        int blocks;
+        mf::PagedAttn a;
+    };
+    auto begin = [&](Shared& k, const FewPlan& s, int min_rows, int max_rows, float* part, bool beside) {
+        k.s = s;
+        k.a = a;
+        k.a.min_rows = min_rows;
+        k.a.max_rows = max_rows;
+        k.a.part = part;
+        k.a.beside = beside;
+        const int r = resident(s.kernel, s.threads, s.smem, &k.blocks);
         if (r) return r;
-        blocks = std::min(blocks, per_sm(s.RT) * num_sms());
-        void* f32_args[] = {&p, &a};
-        void* args[] = {&tk, &tv, &p, &a, &run, &at};
-        e = launch(s.kernel, dim3(blocks), dim3(s.threads), s.smem, st, f32 ? f32_args : args);
-        if (e == cudaSuccess && blocks > 1) {
-            void* jargs[] = {&p, &a, &blocks};
-            e = launch(s.join, dim3(blocks - 1), dim3(256), 0, st, jargs);
-        }
+        k.blocks = std::min(k.blocks, per_sm(s.RT) * num_sms());
+        void* f32_args[] = {&p, &k.a};
+        void* args[] = {&tk, &tv, &p, &k.a, &run, &at};
+        e = launch(s.kernel, dim3(k.blocks), dim3(s.threads), s.smem, st, f32 ? f32_args : args);
         return e == cudaSuccess ? MF_OK : fail(MF_E_CUDA, cudaGetErrorString(e));
     };
+    auto join = [&](Shared& k) {
+        if (k.blocks <= 1) return MF_OK;
+        void* args[] = {&p, &k.a, &k.blocks};
+        e = launch(k.s.join, dim3(k.blocks - 1), dim3(256), 0, st, args);
+        return e == cudaSuccess ? MF_OK : fail(MF_E_CUDA, cudaGetErrorString(e));
+    };
+    Shared chunk = {}, single = {};
+    mf::PagedFa f = {};
+    const size_t rows = (size_t)d->n_tokens * d->n_heads;
     if (chunks && f32) {
-        rc = share_out(few_plan(kv->dtype, D, 64), few ? few_rows : 0, 0x7fffffff, part_chunk);
+        rc = begin(chunk, few_plan(kv->dtype, D, 64), few ? few_rows : 0, 0x7fffffff, part_chunk, false);
         if (rc) return rc;
     } else if (chunks) {
-        mf::PagedFa f = {};
         f.run = run;
         f.at = at;
         f.min_rows = few ? few_rows : 0;
         f.n_split = chunk_split(d->n_tokens, d->n_heads, kv->n_kv_heads);
         if (d->max_len > 0) f.n_split = std::min(f.n_split, std::max(1, d->max_len / (4 * mf::PF_KT)));
-        const size_t rows = (size_t)d->n_tokens * d->n_heads;
         f.part_o = part_chunk;
         f.part_ml = (float2*)(f.part_o + f.n_split * rows * D);
         const void* fn = fa_fn(kv->dtype, D, false);
@@ -435,15 +446,22 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
         if (tiles * kv->n_kv_heads > 0x7fffffffll) return fail(MF_E_UNSUPPORTED, "too many query rows");
         void* args[] = {&tk, &tv, &p, &a, &f};
         e = launch(fn, dim3((unsigned)(tiles * kv->n_kv_heads), (unsigned)f.n_split), dim3(mf::PF_THREADS), smem, st, args);
-        if (e == cudaSuccess && f.n_split > 1) {
-            void* jargs[] = {&p, &a, &f};
-            e = launch(fa_fn(kv->dtype, D, true), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, jargs);
-        }
         if (e != cudaSuccess) return fail(MF_E_CUDA, cudaGetErrorString(e));
     }
-    return few ? share_out(few_plan(kv->dtype, D, std::min<long long>((long long)most * G, chunks ? few_rows : 0x7fffffff)), 0,
-                           chunks ? few_rows : 0x7fffffff, part_few)
-               : MF_OK;
+    if (few) {
+        rc = begin(single, few_plan(kv->dtype, D, std::min<long long>((long long)most * G, chunks ? few_rows : 0x7fffffff)), 0,
+                   chunks ? few_rows : 0x7fffffff, part_few, chunks);
+        if (rc) return rc;
+    }
+    if (chunks && f32) {
+        rc = join(chunk);
+        if (rc) return rc;
+    } else if (chunks && f.n_split > 1) {
+        void* args[] = {&p, &a, &f};
+        e = launch(fa_fn(kv->dtype, D, true), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, args);
+        if (e != cudaSuccess) return fail(MF_E_CUDA, cudaGetErrorString(e));
+    }
+    return few ? join(single) : MF_OK;
 }
 
 int mf_paged_status(int* status, int clear) {

@@ -71,14 +71,16 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS, 2) paged_simt_kernel(const Pa
     float* Vs = Ks + KT * D;
     float* Ss = Vs + KT * D;             // [NG][RT][KT]
     float* alpha_s = Ss + NG * RT * KT;  // [RT]
-    pdl_wait();
-    pdl_launch_dependents();  // after the wait: see paged_join_kernel
+    paged_begin(a);
 
     PagedItem it;
     long long share;
     const long long total = paged_find<RT, KT>(p, a, blockIdx.x, gridDim.x, reinterpret_cast<long long*>(Ks), share, it);
     const long long w0 = blockIdx.x * share, w1 = min(w0 + share, total);
-    if (w0 >= w1) return;
+    if (w0 >= w1) {
+        paged_end(a);
+        return;
+    }
     const int tid = threadIdx.x, grp = tid / GT, tg = tid % GT;
     const int ty = tg / 16, tx = tg % 16;  // rows 4 ty .., keys tx + 16 j, columns 4 tx + 64 j
     const int srow = tid / TPR, sk = tid % TPR;
@@ -254,6 +256,7 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS, 2) paged_simt_kernel(const Pa
         w = it.start + j1;
         if (w < w1) paged_next<RT, KT>(p, a, it);
     }
+    paged_end(a);
 }
 
 }  // namespace mf

@@ -80,14 +80,16 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    pdl_wait();
-    pdl_launch_dependents();  // after the wait: see paged_join_kernel
+    paged_begin(a);
     __syncthreads();
     PagedItem it;
     long long share;
     const long long total = paged_find<RT, KT>(p, a, blockIdx.x, gridDim.x, sh, share, it);
     const long long w0 = blockIdx.x * share, w1 = min(w0 + share, total);
-    if (w0 >= w1) return;
+    if (w0 >= w1) {
+        paged_end(a);
+        return;
+    }
     const unsigned long long deadline = globaltimer_ns() + a.timeout_ns;
     bool failed = false;
 
@@ -382,6 +384,7 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
         }
     }
     if (failed) atomicOr(a.status, 2);
+    paged_end(a);
 }
 
 }  // namespace mf

@@ -27,10 +27,24 @@ struct PagedAttn {
     float scale2;  // softmax scale * log2(e)
     int n_heads, G, window;
     int min_rows, max_rows;  // sequences of other numbers of rows (n_b * G) are another kernel's: min_rows < rows <= max_rows
+    int beside;    // launched behind a chunk kernel that it neither reads nor waits for at its start (paged_begin)
     float* part;   // (O, m, l) of divided items: [2 * grid][RT][D], then [2 * grid][RT][2]
     int* status;   // bit 2: a wait gave up
     unsigned long long timeout_ns;
 };
+
+// A kernel for few rows that follows a chunk kernel of the same call works on
+// other rows, so it starts as that kernel's CTAs leave the SMs and waits for it
+// only at its own end (whoever waits for this one then waits for both). What
+// both read was there before: the chunk kernel lets this one start only after
+// its own wait.
+MF_DEVICE void paged_begin(const PagedAttn& a) {
+    if (!a.beside) pdl_wait();
+    pdl_launch_dependents();  // after the wait: see paged_join_kernel
+}
+MF_DEVICE void paged_end(const PagedAttn& a) {
+    if (a.beside) pdl_wait();
+}
 
 // The keys [lo, hi) that rows [r0, r0 + RT) of a sequence see between them.
 struct PagedSpan {
