@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS, 2) paged_simt_kernel(const Pa
     for (long long w = w0; w < w1;) {
         const int j0 = (int)max(w - it.start, 0ll), j1 = (int)min((long long)it.tiles, w1 - it.start);
         if (j1 <= 0) break;  // only the item's first unit is in this range
-        const int rows = min(RT, it.s.n * a.G - it.r0);
+        const int rows = min(it.step, it.s.n * a.G - it.r0);
         const int kt0 = it.k.lo / KT;
         __syncthreads();
         unsigned long long pages = paged_simt_load<D>(Ks, kb, p, it.b, it.h, (kt0 + j0) * KT, it.k.lo, it.k.hi);
@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS, 2) paged_simt_kernel(const Pa
 #pragma unroll
             for (int e = 0; e < 4 * NC; ++e) o[i][e] = 0.f;
         float m = -INFINITY, l = 0.f;  // of row srow (the same in its threads)
+        const bool busy = 8 * (ty >> 1) < rows;  // a warp has rows of the item: the others skip the products
         const int my_pos = it.s.first + (it.r0 + srow) / a.G;
         const int my_lo = a.window > 0 ? my_pos - a.window + 1 : 0;
 
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS, 2) paged_simt_kernel(const Pa
             __syncthreads();  // K (and Q) are there
             float acc[4][4] = {};
 #pragma unroll 4
-            for (int d = grp * (D / NG); d < (grp + 1) * (D / NG); d += 4) {
+            for (int d = grp * (D / NG); d < (busy ? (grp + 1) * (D / NG) : 0); d += 4) {
                 float4 qv[4], kv[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(Qs + pa_at<D>(4 * ty + i, d));
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(PA_SIMT_THREADS, 2) paged_simt_kernel(const Pa
                 for (int e = 0; e < 4 * NC; ++e) o[i][e] *= al4;
             }
 #pragma unroll 2
-            for (int k = grp * (KT / NG); k < (grp + 1) * (KT / NG); k += 4) {
+            for (int k = grp * (KT / NG); k < (busy ? (grp + 1) * (KT / NG) : 0); k += 4) {
                 float4 pv[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4*>(Ss + pa_at<KT>(4 * ty + i, k));

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
         for (long long w = w0; w < w1;) {
             const int j0 = (int)max(w - it.start, 0ll), j1 = (int)min((long long)it.tiles, w1 - it.start);
             if (j1 <= 0) break;  // only the item's first unit is in this range
-            const int rows = min(RT, it.s.n * a.G - it.r0);
+            const int rows = min(it.step, it.s.n * a.G - it.r0);
             const int key0 = it.k.lo / KT * KT;
             const T* qb = reinterpret_cast<const T*>(a.q) + (long long)it.s.row * a.q_stride + (long long)it.h * a.G * D;
             auto q_row = [&](int r) { return qb + (long long)((it.r0 + r) / a.G) * a.q_stride + (long long)((it.r0 + r) % a.G) * D; };

@@ -1,6 +1,6 @@
 // How the paged attention kernels for few rows share a batch out.
 //
-// An item is a tile of RT query rows (row r of a sequence = token r / G, head
+// An item is a tile of up to RT query rows (row r of a sequence = token r / G, head
 // r % G of the group) of one KV head of one sequence; its work is the number
 // of KT-key tiles that its rows see, after one unit for its beginning and end
 // (queries, join, output: about a tile's time; without it a CTA of 55 one-tile
@@ -60,18 +60,27 @@ MF_DEVICE PagedSpan paged_span(const PagedSeq& s, const PagedAttn& a, int r0, in
 // Number of KT-key tiles of a span; a span without keys still takes one (its rows' zeros are written).
 template <int KT> MF_DEVICE int paged_tiles(const PagedSpan& k) { return max((k.hi + KT - 1) / KT - k.lo / KT, 1); }
 
+// Rows of an item of a sequence of `rows`: as few items as RT allows, of nearly
+// equal size (130 rows are three items of 48, not two of 64 and one of 2: a
+// warp works on 8 rows, and an item counts by its keys alone).
+template <int RT> MF_DEVICE int paged_step(int rows) {
+    const int n = (rows + RT - 1) / RT;
+    return n <= 1 ? RT : min(((rows + n - 1) / n + 7) / 8 * 8, RT);
+}
+
 // Tiles of one KV head of sequence b (0: no rows, or another kernel's)
 template <int RT, int KT> MF_DEVICE int paged_head_work(const PagedSeq& s, const PagedAttn& a) {
     const int rows = s.n * a.G;
     if (rows <= a.min_rows || rows > a.max_rows) return 0;
     int w = 0;
-    for (int r = 0; r < rows; r += RT) w += 1 + paged_tiles<KT>(paged_span(s, a, r, RT));
+    const int step = paged_step<RT>(rows);
+    for (int r = 0; r < rows; r += step) w += 1 + paged_tiles<KT>(paged_span(s, a, r, step));
     return w;
 }
 
 // Item (b, h, r0) of the batch: its tiles are the units [start, start + tiles) of all, after the one at start - 1.
 struct PagedItem {
-    int b, h, r0;
+    int b, h, r0, step;
     long long start;
     int tiles;
     PagedSeq s;
@@ -150,8 +159,9 @@ MF_DEVICE long long paged_find(const PagedKv& p, const PagedAttn& a, int n, int 
         }
         w += (long long)hw * p.n_kv_heads;
     }
-    for (it.r0 = 0;; it.r0 += RT) {
-        it.k = paged_span(it.s, a, it.r0, RT);
+    it.step = paged_step<RT>(it.s.n * a.G);
+    for (it.r0 = 0;; it.r0 += it.step) {
+        it.k = paged_span(it.s, a, it.r0, it.step);
         it.tiles = paged_tiles<KT>(it.k);
         if (at < w + 1 + it.tiles) break;
         w += 1 + it.tiles;
@@ -163,7 +173,7 @@ MF_DEVICE long long paged_find(const PagedKv& p, const PagedAttn& a, int n, int 
 // The item after `it` (only called while work is left).
 template <int RT, int KT> MF_DEVICE void paged_next(const PagedKv& p, const PagedAttn& a, PagedItem& it) {
     it.start += it.tiles + 1;
-    it.r0 += RT;
+    it.r0 += it.step;
     if (it.r0 >= it.s.n * a.G) {
         it.r0 = 0;
         if (++it.h == p.n_kv_heads) {
@@ -171,9 +181,10 @@ template <int RT, int KT> MF_DEVICE void paged_next(const PagedKv& p, const Page
             do {
                 it.s = paged_seq(p, ++it.b);
             } while (it.s.n * a.G <= a.min_rows || it.s.n * a.G > a.max_rows);
+            it.step = paged_step<RT>(it.s.n * a.G);
         }
     }
-    it.k = paged_span(it.s, a, it.r0, RT);
+    it.k = paged_span(it.s, a, it.r0, it.step);
     it.tiles = paged_tiles<KT>(it.k);
 }
 
@@ -197,7 +208,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedKv p, const 
     const int last = mine ? (int)paged_div(it.start + it.tiles - 1, share) : 0;
     pdl_wait();
     if (!mine) return;
-    const int rows = min(RT, it.s.n * a.G - it.r0);
+    const int rows = min(it.step, it.s.n * a.G - it.r0);
     const float* ml = a.part + (long long)2 * grid * RT * D;
     constexpr int V = D / 32, U = 8;
     const int lane = threadIdx.x & 31;
