@@ -319,11 +319,11 @@ int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* d, voi
     r.n_heads = d->n_heads;
     r.d_rot = d->d_rot;
     r.interleaved = d->interleaved != 0;
-    // Heads per warp: the angles cost about as much as a few heads, so a warp
-    // takes more heads as soon as the warps still fill the SMs.
+    // Heads per warp: the angles cost about as much as eight heads, so a warp
+    // takes more than its four at a time as soon as the warps still fill the SMs.
     const int H = d->n_heads + 2 * kv->n_kv_heads;
     const long long warps = (long long)num_sms() * 32;
-    r.hpw = (int)std::min<long long>(std::max<long long>((long long)d->n_tokens * H / warps, 1), 16);
+    r.hpw = (int)std::min<long long>(std::max<long long>((long long)d->n_tokens * H / warps / 4 * 4, 4), 32);
     const long long units = (long long)d->n_tokens * ((H + r.hpw - 1) / r.hpw);
     const long long blocks = (units + mf::ROPE_WARPS - 1) / mf::ROPE_WARPS;
     if (blocks > 0x7fffffffll) return fail(MF_E_UNSUPPORTED, "too many rows");
