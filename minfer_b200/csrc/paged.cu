@@ -232,11 +232,33 @@ int resident(const void* fn, int threads, size_t smem, int* blocks) {
 // Blocks per SM that the workspace of the kernels for few rows is sized for.
 int per_sm(int RT) { return RT == 16 ? 4 : 2; }
 
-// Shares of the keys in which the chunk kernel works when its row tiles alone
-// leave SMs idle (1: none).
-int chunk_split(int n_tokens, int n_heads, int n_kv_heads) {
+// Shares of the keys in which the chunk kernel works, so that a batch of few
+// row tiles fills the SMs: the number with the shortest estimate. A CTA takes
+// about 1.9 us per tile of 128 keys and as long as three tiles to begin and
+// end; joining n shares reads and writes n fp32 rows of D per query row.
+// (100 row tiles after 8192 keys: 3 shares, two rounds of a third each, 0.8 of
+// the time of one; 128 row tiles after 29184: one.)
+constexpr int MAX_SPLIT = 16;
+int chunk_split(int n_tokens, int n_heads, int n_kv_heads, int D, long long keys) {
     const long long ctas = ((long long)n_tokens * (n_heads / n_kv_heads) + mf::PF_ROWS - 1) / mf::PF_ROWS * n_kv_heads;
-    return (int)std::min<long long>(std::max<long long>(num_sms() / ctas, 1), 16);
+    const double tiles = std::max(1.0, (double)keys / mf::PF_KT), row_us = 2.0 * n_tokens * n_heads * D * 4 / 6e6;
+    const int sms = num_sms();
+    int best = 1;
+    double least = 0;
+    for (int n = 1; n <= MAX_SPLIT && (n == 1 || (ctas * n <= 4ll * sms && tiles >= 2.0 * n)); ++n) {
+        const double us = (double)((ctas * n + sms - 1) / sms) * (tiles / n + 3) * 1.9 + (n > 1 ? 4 + n * row_us : 0);
+        if (n == 1 || us < least) {
+            best = n;
+            least = us;
+        }
+    }
+    return best;
+}
+// Query rows x shares are bounded by the rule above (at most 4 CTAs of 256 rows per SM, or one share).
+size_t split_bytes(int n_tokens, int n_heads, int n_kv_heads, int D) {
+    const long long ctas = ((long long)n_tokens * (n_heads / n_kv_heads) + mf::PF_ROWS - 1) / mf::PF_ROWS * n_kv_heads;
+    const long long n = std::min<long long>(4ll * num_sms() / ctas, MAX_SPLIT);
+    return n <= 1 ? 0 : (size_t)n * n_tokens * n_heads * (D + 2) * sizeof(float);
 }
 
 template <typename T, int D> const void* fa_fn2(bool join) {
@@ -334,10 +356,9 @@ int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* d, voi
 }
 
 size_t mf_paged_attention_workspace_bytes(int n_tokens, int n_heads, int n_kv_heads, int d_head, int dtype) {
-    if (n_tokens <= 0 || n_heads <= 0 || n_kv_heads <= 0 || (d_head != 64 && d_head != 128) || !known_dtype(dtype)) return 0;
+    if (n_tokens <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads < n_kv_heads || (d_head != 64 && d_head != 128) || !known_dtype(dtype)) return 0;
     const size_t few = part_bytes(num_sms(), 64, d_head);  // 4 blocks per SM of 16 rows, 2 of 32
-    const size_t split = (size_t)chunk_split(n_tokens, n_heads, n_kv_heads) * n_tokens * n_heads * (d_head + 2) * sizeof(float);
-    return few + (dtype == MF_F32 ? part_bytes(2 * num_sms(), 64, d_head) : split);
+    return few + (dtype == MF_F32 ? part_bytes(2 * num_sms(), 64, d_head) : split_bytes(n_tokens, n_heads, n_kv_heads, d_head));
 }
 
 int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void* stream) {
@@ -431,8 +452,10 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
         f.run = run;
         f.at = at;
         f.min_rows = few ? few_rows : 0;
-        f.n_split = chunk_split(d->n_tokens, d->n_heads, kv->n_kv_heads);
-        if (d->max_len > 0) f.n_split = std::min(f.n_split, std::max(1, d->max_len / (4 * mf::PF_KT)));
+        long long keys = (long long)p.max_pages * p.page_size;  // that a row tile sees at most
+        if (d->max_len > 0) keys = std::min<long long>(keys, d->max_len);
+        if (d->window > 0) keys = std::min<long long>(keys, (long long)d->window + mf::PF_ROWS / G);
+        f.n_split = chunk_split(d->n_tokens, d->n_heads, kv->n_kv_heads, D, keys);
         f.part_o = part_chunk;
         f.part_ml = (float2*)(f.part_o + f.n_split * rows * D);
         const void* fn = fa_fn(kv->dtype, D, false);

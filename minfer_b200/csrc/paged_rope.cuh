@@ -20,7 +20,8 @@
 // by two; so rotating needs no exchange, and the norm three shuffles for four
 // heads. (With a head across the warp the sums and exchanges took 90
 // instructions a head, more time than its 768 bytes: 42 us for the chunk below.)
-// Measured: 156 MB (fp32 rows of 80 heads to bf16) in 28 us, 0.85 of the copy rate.
+// Measured: 156 MB (fp32 rows of 80 heads to bf16) in 34 us, 0.70 of the copy
+// rate; 33 with a 64-register limit (but 4.6 us instead of 3.7 for 64 tokens).
 #pragma once
 
 #include "paged.cuh"
@@ -45,7 +46,7 @@ constexpr int ROPE_WARPS = 8;
 constexpr int ROPE_HEADS = 4;  // heads of a warp at a time
 
 template <typename X, typename T, int D>
-__global__ void __launch_bounds__(ROPE_WARPS * 32) paged_rope_kernel(const PagedKv p, const PagedRope r) {
+__global__ void __launch_bounds__(ROPE_WARPS * 32, 3) paged_rope_kernel(const PagedKv p, const PagedRope r) {
     constexpr int NS = D / 64;  // pairs of blocks per lane
     constexpr int NA = 4 * NS;  // angles per lane
     pdl_launch_dependents();
