@@ -306,9 +306,10 @@ int mf_rope_freqs(double* out, int d_rot, double base, int scaling, double facto
     return MF_OK;
 }
 
-int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* d, void* stream) {
+static int rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* d, void* stream) {
     mf::PagedKv p;
-    if (!d) return fail(MF_E_INVALID, "null argument");
+    if (!kv || !d) return fail(MF_E_INVALID, "null argument");
+    if (d->n_tokens == 0 || kv->n_seqs == 0) return MF_OK;  // nothing to do (empty tensors have no address)
     int rc = resolve_kv(kv, d->n_tokens, &p);
     if (rc) return rc;
     if (!d->q_out || !d->qkv || (!d->freqs && d->d_rot > 0)) return fail(MF_E_INVALID, "null argument");
@@ -331,7 +332,6 @@ int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* d, voi
         return fail(MF_E_INVALID, "qkv and q_out: rows must be 16-byte aligned and not overlap");
     if (!aligned(d->freqs, 8) || !aligned(d->q_norm_w, 4) || !aligned(d->k_norm_w, 4) || !aligned(d->positions, 4))
         return fail(MF_E_INVALID, "misaligned table");
-    if (d->n_tokens == 0 || kv->n_seqs == 0) return MF_OK;
     r.freqs = d->freqs;
     r.q_norm_w = d->q_norm_w;
     r.k_norm_w = d->k_norm_w;
@@ -361,9 +361,10 @@ size_t mf_paged_attention_workspace_bytes(int n_tokens, int n_heads, int n_kv_he
     return few + (dtype == MF_F32 ? part_bytes(2 * num_sms(), 64, d_head) : split_bytes(n_tokens, n_heads, n_kv_heads, d_head));
 }
 
-int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void* stream) {
+static int attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void* stream) {
     mf::PagedKv p;
-    if (!d) return fail(MF_E_INVALID, "null argument");
+    if (!kv || !d) return fail(MF_E_INVALID, "null argument");
+    if (d->n_tokens == 0 || kv->n_seqs == 0) return MF_OK;  // nothing to do (empty tensors have no address)
     int rc = resolve_kv(kv, d->n_tokens, &p);
     if (rc) return rc;
     if (!d->out || !d->q) return fail(MF_E_INVALID, "null argument");
@@ -382,14 +383,14 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
     if (a.out_stride < (long long)d->n_heads * D || a.q_stride < (long long)d->n_heads * D || a.out_stride % u ||
         a.q_stride % u || !aligned(d->out, 16) || !aligned(d->q, 16))
         return fail(MF_E_INVALID, "q and out: rows must be 16-byte aligned and not overlap");
-    if (d->n_tokens == 0 || kv->n_seqs == 0) return MF_OK;
     if (!d->workspace || !aligned(d->workspace, 256) ||
         d->workspace_bytes < mf_paged_attention_workspace_bytes(d->n_tokens, d->n_heads, kv->n_kv_heads, D, kv->dtype))
         return fail(MF_E_INVALID, "workspace missing, too small or not 256-byte aligned");
     a.scale2 = (d->scale == 0.f ? 1.0f / sqrtf((float)D) : d->scale) * 1.4426950408889634f;
     a.n_heads = d->n_heads;
     a.G = G;
-    a.window = d->window;
+    // a window as long as the table hides nothing; beyond 2^30 its arithmetic would leave 32 bits
+    a.window = d->window >= std::min<long long>((long long)p.max_pages * p.page_size, 1 << 30) ? 0 : d->window;
     const int most = std::min(d->max_new > 0 ? d->max_new : d->n_tokens, d->n_tokens);
     cudaStream_t st = mf::resolve_stream(stream);
 
@@ -454,7 +455,7 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
         f.min_rows = few ? few_rows : 0;
         long long keys = (long long)p.max_pages * p.page_size;  // that a row tile sees at most
         if (d->max_len > 0) keys = std::min<long long>(keys, d->max_len);
-        if (d->window > 0) keys = std::min<long long>(keys, (long long)d->window + mf::PF_ROWS / G);
+        if (a.window > 0) keys = std::min<long long>(keys, (long long)a.window + mf::PF_ROWS / G);
         f.n_split = chunk_split(d->n_tokens, d->n_heads, kv->n_kv_heads, D, keys);
         f.part_o = part_chunk;
         f.part_ml = (float2*)(f.part_o + f.n_split * rows * D);
@@ -485,6 +486,23 @@ int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void*
         if (e != cudaSuccess) return fail(MF_E_CUDA, cudaGetErrorString(e));
     }
     return few ? join(single) : MF_OK;
+}
+
+// No C++ exception leaves the library (the caches of launch attributes allocate).
+int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* desc, void* stream) {
+    try {
+        return rope_append(kv, desc, stream);
+    } catch (...) {
+        return fail(MF_E_OOM, "out of host memory");
+    }
+}
+
+int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* desc, void* stream) {
+    try {
+        return attention(kv, desc, stream);
+    } catch (...) {
+        return fail(MF_E_OOM, "out of host memory");
+    }
 }
 
 int mf_paged_status(int* status, int clear) {

@@ -15,12 +15,14 @@ int record_error(int code, const char* msg);
 cudaStream_t resolve_stream(void* stream);
 }  // namespace mf
 
-extern "C" int mf_sample_batch(int* ids, float* probs, const void* logits, int dtype, long long ld, int n_rows, int vocab,
+namespace {
+int sample_batch(int* ids, float* probs, const void* logits, int dtype, long long ld, int n_rows, int vocab,
                                const float* draws, const float* temp, const int* top_k, const float* top_p,
                                const float* min_p, void* stream) {
     auto fail = [](int code, const char* msg) { return mf::record_error(code, msg); };
+    if (n_rows == 0) return MF_OK;  // nothing to do (empty tensors have no address)
     if (!ids || !logits || !draws || !temp || !top_k || !top_p || !min_p) return fail(MF_E_INVALID, "null argument");
-    if (n_rows < 0 || vocab <= 0 || ld < vocab) return fail(MF_E_INVALID, "need n_rows >= 0, vocab > 0 and ld >= vocab");
+    if (n_rows < 0 || vocab <= 0 || ld < vocab) return fail(MF_E_INVALID, "need n_rows > 0, vocab > 0 and ld >= vocab");
     if (vocab > mf::SB_MAX_VOCAB) return fail(MF_E_UNSUPPORTED, "vocabulary above 2^18");
     const void* fn = dtype == MF_F32    ? (const void*)&mf::sample_batch_kernel<float>
                      : dtype == MF_F16  ? (const void*)&mf::sample_batch_kernel<__half>
@@ -32,7 +34,6 @@ extern "C" int mf_sample_batch(int* ids, float* probs, const void* logits, int d
         (((uintptr_t)ids | (uintptr_t)probs | (uintptr_t)draws | (uintptr_t)temp | (uintptr_t)top_k | (uintptr_t)top_p |
           (uintptr_t)min_p) & 3) != 0)
         return fail(MF_E_INVALID, "misaligned argument");
-    if (n_rows == 0) return MF_OK;
     // Blocks per row: as many as keep a block's slice at 4096 logits or more, at most 8.
     int cluster = 1;
     while (cluster < mf::SB_MAX_CLUSTER && (vocab + cluster - 1) / cluster > 4096) cluster *= 2;
@@ -80,4 +81,15 @@ extern "C" int mf_sample_batch(int* ids, float* probs, const void* logits, int d
     void* args[] = {&a};
     cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
     return e == cudaSuccess ? MF_OK : fail(MF_E_CUDA, cudaGetErrorString(e));
+}
+}  // namespace
+
+extern "C" int mf_sample_batch(int* ids, float* probs, const void* logits, int dtype, long long ld, int n_rows, int vocab,
+                               const float* draws, const float* temp, const int* top_k, const float* top_p,
+                               const float* min_p, void* stream) {
+    try {
+        return sample_batch(ids, probs, logits, dtype, ld, n_rows, vocab, draws, temp, top_k, top_p, min_p, stream);
+    } catch (...) {
+        return mf::record_error(MF_E_OOM, "out of host memory");
+    }
 }

@@ -216,7 +216,8 @@ def _rows(t: torch.Tensor, name: str, dtype, device: int, n: int, width: int) ->
             return p, width
     else:
         stride = t.stride()
-        if shape[0] == n and inner == width and stride[-1] == 1 and (dims == 2 or stride[1] == shape[2]):
+        if (shape[0] == n and inner == width and stride[-1] == 1 and (dims == 2 or stride[1] == shape[2] or shape[1] == 1)
+                and (n <= 1 or stride[0] >= width)):
             return p, stride[0] if n > 1 else width
     raise ValueError(f"{name}: expected {n} rows of {width} contiguous elements, got {tuple(shape)} with strides {t.stride()}")
 
@@ -232,11 +233,15 @@ def _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens) -> tuple[bytes, in
     strides = k_pages.stride()
     if v_pages.shape != shape or v_pages.stride() != strides or strides[3] != 1:
         raise ValueError("k_pages and v_pages: expected the same shape and strides, heads contiguous")
+    # the stride of an extent of one says nothing (0: the default); otherwise 0 is an expanded tensor
+    strides = strides[0] if n_pages > 1 else 0, strides[1] if heads > 1 else 0, strides[2]
+    if (n_pages > 1 and strides[0] <= 0) or (heads > 1 and strides[1] <= 0) or strides[2] <= 0:
+        raise ValueError("k_pages and v_pages: pages, heads and rows must not be expanded")
     table = _tensor(page_table, "page_table", torch.int32, device, 2)
     n_seqs, max_pages = page_table.shape
     table_stride, inner = page_table.stride()
-    if max_pages > 1 and inner != 1:
-        raise ValueError("page_table: expected contiguous rows")
+    if (max_pages > 1 and inner != 1) or (n_seqs > 1 and table_stride < max_pages):
+        raise ValueError("page_table: expected contiguous rows that do not overlap")
     return _KV.pack(k_pages.data_ptr(), vp, strides[0], strides[1], strides[2], table,
                     _vector(q_start, "q_start", torch.int32, device, n_seqs + 1),
                     _vector(kv_lens, "kv_lens", torch.int32, device, n_seqs),

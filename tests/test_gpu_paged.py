@@ -8,6 +8,7 @@ import torch
 from minfer_b200 import ops
 from minfer_b200._lib import MinferError
 import paged_ref as ref
+from test_gpu_sample_batch import rule as sampling_rule_64
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -309,6 +310,80 @@ def test_python_refusals_on_gpu():
     ops.paged_attention(**good)
 
 
+def test_expanded_tensors_are_refused():
+    """A stride of 0 must not be read as "contiguous"."""
+    b = ref.Batch([(1, 20), (1, 30)], 4, 2, 128, 16, BF16)
+    q, out = b.q(), torch.empty(2, 4, 128, dtype=BF16, device="cuda")
+    good = dict(out=out, q=q, k_pages=b.k, v_pages=b.v, page_table=b.table, q_start=b.q_start, kv_lens=b.lens)
+    one = b.k[:1].expand(b.n_pages, -1, -1, -1)
+    head = b.k[:, :1].expand(-1, 2, -1, -1)
+    row = b.k[:, :, :1].expand(-1, -1, 16, -1)
+    for change in (dict(q=q[:1].expand(2, -1, -1)), dict(out=out[:1].expand(2, -1, -1)), dict(k_pages=one, v_pages=one), dict(k_pages=head, v_pages=head),
+                   dict(k_pages=row, v_pages=row), dict(page_table=b.table[:1].expand(2, -1)), dict(q=torch.zeros(2, 128, 4, dtype=BF16, device="cuda").transpose(1, 2))):
+        with pytest.raises(ValueError):
+            ops.paged_attention(**{**good, **change})
+    with pytest.raises(ValueError):
+        ops.paged_rope_append(q, b.k, b.v, b.table, torch.zeros(1, 8 * 128, device="cuda").expand(2, -1), b.q_start, b.lens, torch.zeros(64, dtype=torch.float64, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [t for t, _ in TYPES], ids=[n for _, n in TYPES])
+def test_extents_of_one(dtype):
+    """One page, one head, one sequence, one token: whatever strides torch gives them."""
+    for nhd in (False, True):
+        b = ref.Batch([(1, 13)], 3, 1, 64, 16, dtype, nhd=nhd, spare=0)
+        assert b.n_pages == 1
+        check_attention(b)
+        b.k, b.v = (x.as_strided(x.shape, (5, 7, *x.stride()[2:])) for x in (b.k, b.v))
+        check_attention(b)
+    b = ref.Batch([(1, 100)], 2, 2, 128, 8, dtype, nhd=True, spare=0)
+    check_attention(b)
+
+
+def test_nothing_to_do():
+    """No tokens, or no sequences: no error, nothing written."""
+    b = ref.Batch([(1, 20)], 4, 2, 128, 16, BF16, gap=(0, 2))
+    f = ops.rope_freqs(128, 1e6)[0].cuda()
+    k = b.k.clone()
+    none = torch.empty(0, 4, 128, dtype=BF16, device="cuda")
+    ops.paged_attention(none, none, *b.args())
+    ops.paged_rope_append(none, *b.args()[:3], torch.empty(0, 8 * 128, device="cuda"), b.q_start, b.lens, f)
+    out = torch.full((3, 4, 128), SENTINEL, dtype=BF16, device="cuda")
+    empty = (b.k, b.v, b.table[:0], b.q_start[:1], b.lens[:0])
+    ops.paged_attention(out, torch.zeros_like(out), *empty)
+    ops.paged_rope_append(out, *empty[:3], torch.zeros(3, 8 * 128, device="cuda"), *empty[3:], f)
+    assert (out == SENTINEL).all() and torch.equal(b.k.nan_to_num(), k.nan_to_num())
+    # sequences without new tokens, rows of nobody
+    ops.paged_attention(out, torch.zeros_like(out), b.k, b.v, b.table, torch.zeros(2, dtype=torch.int32, device="cuda"), b.lens)
+    assert (out == SENTINEL).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_starts_and_lengths_out_of_range(dtype):
+    """Starts past the call's rows and lengths past the table are clamped; a start that decreases gives no rows."""
+    b = ref.Batch([(2, 48), (50, 90), (1, 7)], 4, 2, 128, 16, dtype, seed=30)  # the first fills its pages
+    q = b.q()
+    want = run_attention(b, q)
+    b.q_start[-1] = 10 ** 6
+    assert torch.equal(run_attention(b, q), want)
+    b.q_start[-1] = -5  # the last sequence has no rows
+    got = run_attention(b, q)
+    assert torch.equal(got[:52], want[:52]) and (got[52] == SENTINEL).all()
+    b.q_start[-1] = 53
+    b.lens[0] = 2 ** 31 - 1  # clamped to the table's capacity: positions without a page hold no keys
+    b.seqs[0] = (2, b.max_pages * b.page)
+    check_attention(b, q)
+    b.lens[0] = -7
+    b.seqs[0] = (2, 0)
+    check_attention(b, q)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30, 400])
+def test_windows_longer_than_everything(window):
+    b = ref.Batch([(1, 90), (60, 200), (5, 3)], 4, 2, 128, 16, BF16, seed=31)
+    q = b.q()
+    assert torch.equal(run_attention(b, q, window=window), run_attention(b, q))
+
+
 def step(b, qkv, f, q, out, ws, **kw):
     ops.paged_rope_append(q, b.k, b.v, b.table, qkv, b.q_start, b.lens, f)
     ops.paged_attention(out, q, *b.args(), workspace=ws, **kw)
@@ -369,3 +444,58 @@ def test_same_call_same_bits():
     first = run_attention(b, q)
     for _ in range(5):
         assert torch.equal(run_attention(b, q), first)
+
+
+def test_batched_decoding_with_sampling():
+    """The three operators as a batch is served: prompts of three sequences in one call, then single tokens, each id
+    sampled from the logits of the last position; against the same steps in 64 bits."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(40)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    vocab, hq, hkv, d, page = 997, 4, 2, 64, 16
+    emb, wqkv, wo = r(vocab, 96), r(96, (hq + 2 * hkv) * d) / 10, r(hq * d, vocab) / 4
+    qw, kw = 1 + 0.1 * r(d), 1 + 0.1 * r(d)
+    f, m = ops.rope_freqs(d, 1e4, "yarn", 2.0, 512)
+    f = f.cuda()
+    prompts = [torch.randint(0, vocab, (n,), generator=g, device="cuda").tolist() for n in (5, 40, 17)]
+    k, v = (torch.full((20, hkv, page, d), math.nan, device="cuda") for _ in range(2))
+    table = torch.randperm(20, generator=g, device="cuda").to(torch.int32)[:15].view(3, 5).contiguous()
+    temp, top_k = torch.tensor([0.0, 0.8, 1.2], device="cuda"), torch.tensor([0, 50, 0], dtype=torch.int32, device="cuda")
+    top_p, min_p = torch.tensor([1.0, 0.9, 0.95], device="cuda"), torch.tensor([0.0, 0.0, 0.02], device="cuda")
+    lens = [0, 0, 0]
+    seqs = [list(p) for p in prompts]
+    for n_step in range(6):
+        new = [s[n:] for s, n in zip(seqs, lens)]
+        lens = [len(s) for s in seqs]
+        start = [0]
+        for n in new:
+            start.append(start[-1] + len(n))
+        tok = torch.tensor(sum(new, []), device="cuda")
+        q_start, kv_lens = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (start, lens))
+        qkv = emb[tok] @ wqkv
+        q, out = torch.empty(len(tok), hq, d, device="cuda"), torch.empty(len(tok), hq, d, device="cuda")
+        ops.paged_rope_append(q, k, v, table, qkv, q_start, kv_lens, f, mscale=m, q_norm_w=qw, k_norm_w=kw)
+        ops.paged_attention(out, q, k, v, table, q_start, kv_lens)
+        last = q_start[1:].long() - 1
+        logits = out[last].view(3, -1) @ wo
+        draws, ids, probs = torch.rand(3, generator=g, device="cuda"), torch.empty(3, dtype=torch.int32, device="cuda"), torch.empty(3, device="cuda")
+        ops.sample_batch(ids, logits, draws, temp, top_k, top_p, min_p, probs=probs)
+        for b in range(3):  # the whole sequence from its ids, in 64 bits
+            x = (emb[torch.tensor(seqs[b], device="cuda")].double() @ wqkv.double()).view(-1, hq + 2 * hkv, d)
+            y = x[:, :hq + hkv]
+            y = y / torch.sqrt((y ** 2).mean(-1, keepdim=True) + 1e-6) * torch.cat([qw.double().expand(hq, d), kw.double().expand(hkv, d)])
+            ang = 2 * math.pi * torch.arange(len(y), device="cuda").double()[:, None, None] * f
+            a, z = y[..., :d // 2], y[..., d // 2:]
+            y = m * torch.cat([a * torch.cos(ang) - z * torch.sin(ang), z * torch.cos(ang) + a * torch.sin(ang)], -1)
+            kk, vv = y[:, hq:].repeat_interleave(hq // hkv, 1), x[:, hq + hkv:].repeat_interleave(hq // hkv, 1)
+            p = torch.softmax(torch.einsum("hd,khd->hk", y[-1, :hq], kk) / math.sqrt(d), -1)
+            lg = torch.einsum("hk,khd->hd", p, vv).reshape(-1) @ wo.double()
+            assert (logits[b].double() - lg).abs().max() < 1e-4 * lg.abs().max()  # fp32 products of 96 and 256 terms
+            want, prob = sampling_rule_64(lg.float().cpu().numpy(), draws[b].item(), temp[b].item(), top_k[b].item(), top_p[b].item(), min_p[b].item())
+            assert ids[b].item() == want and abs(probs[b].item() - prob) < 1e-3
+            seqs[b].append(want)
+    assert ops.paged_status() == 0
+
+
+def test_no_wait_gave_up():
+    assert ops.paged_status(clear=False) == 0

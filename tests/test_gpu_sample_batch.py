@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from minfer_b200 import ops
+from minfer_b200._lib import MinferError
 
 pytestmark = pytest.mark.gpu
 
@@ -142,6 +143,29 @@ def test_bad_parameters_have_a_meaning():
     assert run(x, 0.9, 1.0, 0, 1.0, 7.0)[0] == [1]
     with pytest.raises(ValueError):
         ops.sample_batch(torch.zeros(1, dtype=torch.int64, device="cuda"), x, *[torch.zeros(1, device="cuda")] * 5)
+
+
+def test_no_rows():
+    ids = torch.empty(0, dtype=torch.int32, device="cuda")
+    f = torch.empty(0, device="cuda")
+    ops.sample_batch(ids, torch.empty(0, 100, device="cuda"), f, f, ids, f, f, probs=f)
+    with pytest.raises(MinferError):  # rows that overlap
+        x = torch.zeros(1, 9, device="cuda").expand(3, -1)
+        ops.sample_batch(torch.zeros(3, dtype=torch.int32, device="cuda"), x, *[torch.zeros(3, device="cuda")] * 2, torch.zeros(3, dtype=torch.int32, device="cuda"),
+                         *[torch.zeros(3, device="cuda")] * 2)
+
+
+def test_crowded_bins():
+    """Thousands of candidates within a sixteenth of the border: the descent that does not fit one block."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(6)
+    x = 5 + torch.rand(4, 30000, generator=g, device="cuda") * 0.05
+    x[1, :9000] = x[1, 0]
+    x[2] = x[2].to(torch.bfloat16).float()
+    x[3, ::3] -= 40
+    r = torch.rand(4, generator=g, device="cuda")
+    for temp, top_k, top_p, min_p in ((1.0, 0, 0.5, 0.0), (0.01, 0, 0.999, 0.0), (1.0, 12000, 1.0, 0.0), (2.0, 12000, 0.7, 0.97), (1.0, 0, 1.0, 0.98), (0.3, 29999, 0.3, 0.0)):
+        check(x, r, temp, top_k, top_p, min_p)
 
 
 def test_draws_follow_the_distribution():
