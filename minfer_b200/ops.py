@@ -188,20 +188,19 @@ _KV = Struct("@PPqqqPPPiiiiiiii")
 _ROPE = Struct("@PqPqiiiiiffPPPP0P")
 _ATTN = Struct("@PqPqiifiiiPN")
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # absent on builds without CUDA
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _tensor(t: torch.Tensor, name: str, dtype, device: int, dims: int) -> int:
-    """Address of a tensor on CUDA device `device` with the given dtype and rank; strides are the caller's business."""
-    if t.dtype is not dtype or t.dim() != dims or t.get_device() != device:
-        raise ValueError(f"{name}: expected a {dims}-d {dtype} tensor on cuda:{device}, got {t.dim()}-d {t.dtype} on {t.device}")
-    return t.data_ptr()
+def _refuse(t: torch.Tensor, name: str, want: str):
+    raise ValueError(f"{name}: expected {want}, got {tuple(t.shape)} {t.dtype} with strides {t.stride()} on {t.device}")
 
 
 def _vector(t: torch.Tensor | None, name: str, dtype, device: int, n: int) -> int:
+    """Address of n contiguous elements (0 for None)."""
     if t is None:
         return 0
-    if t.dtype is not dtype or t.dim() != 1 or t.get_device() != device or t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"{name}: expected {n} contiguous {dtype} elements on cuda:{device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if t.dtype is not dtype or t.get_device() != device or t.shape != (n,) or not t.is_contiguous():
+        _refuse(t, name, f"{n} contiguous {dtype} elements on cuda:{device}")
     return t.data_ptr()
 
 
@@ -209,52 +208,55 @@ def _rows(t: torch.Tensor, name: str, dtype, device: int, n: int, width: int) ->
     """Address and row stride of n rows of `width` contiguous elements: [n, width], or [n, heads, d_head]."""
     shape = t.shape
     dims = len(shape)
-    p = _tensor(t, name, dtype, device, 3 if dims == 3 else 2)
-    inner = shape[1] if dims == 2 else shape[1] * shape[2]
-    if t.is_contiguous():
-        if shape[0] == n and inner == width:
-            return p, width
-    else:
+    if (t.dtype is dtype and t.get_device() == device and 2 <= dims <= 3 and shape[0] == n
+            and (shape[1] if dims == 2 else shape[1] * shape[2]) == width):
+        if t.is_contiguous():
+            return t.data_ptr(), width
         stride = t.stride()
-        if (shape[0] == n and inner == width and stride[-1] == 1 and (dims == 2 or stride[1] == shape[2] or shape[1] == 1)
-                and (n <= 1 or stride[0] >= width)):
-            return p, stride[0] if n > 1 else width
-    raise ValueError(f"{name}: expected {n} rows of {width} contiguous elements, got {tuple(shape)} with strides {t.stride()}")
+        if stride[-1] == 1 and (dims == 2 or stride[1] == shape[2] or shape[1] == 1) and (n <= 1 or stride[0] >= width):
+            return t.data_ptr(), stride[0] if n > 1 else width
+    _refuse(t, name, f"{n} rows of {width} contiguous {dtype} elements on cuda:{device}")
+
+
+def _width(t: torch.Tensor) -> int:
+    shape = t.shape
+    return shape[1] if len(shape) == 2 else shape[1] * shape[2] if len(shape) == 3 else -1
 
 
 def _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens) -> tuple[bytes, int, int, int, int]:
     """The cache's packed description, its device, KV heads, head width and dtype code."""
-    dtype, device, shape = k_pages.dtype, k_pages.get_device(), k_pages.shape
+    dtype, device, shape, strides = k_pages.dtype, k_pages.get_device(), k_pages.shape, k_pages.stride()
     code = _CODES.get(dtype)
-    if code is None or len(shape) != 4 or device < 0:
-        raise ValueError("k_pages: expected a CUDA tensor [n_pages, n_kv_heads, page_size, d_head] of float32, float16 or bfloat16")
-    vp = _tensor(v_pages, "v_pages", dtype, device, 4)
+    if code is None or len(shape) != 4 or device < 0 or strides[3] != 1:
+        _refuse(k_pages, "k_pages", "a CUDA tensor [n_pages, n_kv_heads, page_size, d_head] of float32, float16 or bfloat16, heads contiguous")
+    if v_pages.dtype is not dtype or v_pages.get_device() != device or v_pages.shape != shape or v_pages.stride() != strides:
+        _refuse(v_pages, "v_pages", "the dtype, device, shape and strides of k_pages")
     n_pages, heads, size, d = shape
-    strides = k_pages.stride()
-    if v_pages.shape != shape or v_pages.stride() != strides or strides[3] != 1:
-        raise ValueError("k_pages and v_pages: expected the same shape and strides, heads contiguous")
     # the stride of an extent of one says nothing (0: the default); otherwise 0 is an expanded tensor
-    strides = strides[0] if n_pages > 1 else 0, strides[1] if heads > 1 else 0, strides[2]
-    if (n_pages > 1 and strides[0] <= 0) or (heads > 1 and strides[1] <= 0) or strides[2] <= 0:
-        raise ValueError("k_pages and v_pages: pages, heads and rows must not be expanded")
-    table = _tensor(page_table, "page_table", torch.int32, device, 2)
-    n_seqs, max_pages = page_table.shape
-    table_stride, inner = page_table.stride()
-    if (max_pages > 1 and inner != 1) or (n_seqs > 1 and table_stride < max_pages):
-        raise ValueError("page_table: expected contiguous rows that do not overlap")
-    return _KV.pack(k_pages.data_ptr(), vp, strides[0], strides[1], strides[2], table,
+    page_stride = strides[0] if n_pages > 1 else 0
+    head_stride = strides[1] if heads > 1 else 0
+    if (n_pages > 1 and page_stride <= 0) or (heads > 1 and head_stride <= 0) or strides[2] <= 0:
+        _refuse(k_pages, "k_pages", "pages, heads and rows that are not expanded")
+    table_shape, table_strides = page_table.shape, page_table.stride()
+    if (page_table.dtype is not torch.int32 or page_table.get_device() != device or len(table_shape) != 2
+            or (table_shape[1] > 1 and table_strides[1] != 1) or (table_shape[0] > 1 and table_strides[0] < table_shape[1])):
+        _refuse(page_table, "page_table", f"int32 rows on cuda:{device}, each contiguous, that do not overlap")
+    n_seqs, max_pages = table_shape
+    return _KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), page_stride, head_stride, strides[2], page_table.data_ptr(),
                     _vector(q_start, "q_start", torch.int32, device, n_seqs + 1),
                     _vector(kv_lens, "kv_lens", torch.int32, device, n_seqs),
-                    table_stride if n_seqs > 1 else max_pages, max_pages, n_pages, size, n_seqs, heads, d, code), device, heads, d, code
+                    table_strides[0] if n_seqs > 1 else max_pages, max_pages, n_pages, size, n_seqs, heads, d, code), device, heads, d, code
 
 
 def _on(device: int, fn, *args) -> None:
     """fn(*args, stream) on torch's current stream of CUDA device `device`."""
-    if torch.cuda.current_device() == device:
-        check(fn(*args, _raw_stream(device) or _CUDA_STREAM_LEGACY))
+    if _current_device() == device:
+        rc = fn(*args, _raw_stream(device) or _CUDA_STREAM_LEGACY)
     else:
         with torch.cuda.device(device):
-            check(fn(*args, _raw_stream(device) or _CUDA_STREAM_LEGACY))
+            rc = fn(*args, _raw_stream(device) or _CUDA_STREAM_LEGACY)
+    if rc < 0:
+        check(rc)
 
 
 def rope_freqs(d_rot: int, base: float, scaling: str = "none", factor: float = 1.0, orig_ctx: float = 0.0,
@@ -281,7 +283,7 @@ def paged_rope_append(q_out, k_pages, v_pages, page_table, qkv, q_start, kv_lens
     [d_rot / 2] in turns per position (rope_freqs). Rows of no sequence, and the rest of the pages, stay as they are."""
     kv, device, heads, d, _ = _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens)
     n, half = qkv.shape[0], freqs.shape[0]
-    q_width = q_out.shape[1] * (q_out.shape[2] if q_out.dim() == 3 else 1)
+    q_width = _width(q_out)
     x_code = _CODES.get(qkv.dtype)
     if x_code is None:
         raise ValueError(f"qkv: unsupported dtype {qkv.dtype}")
@@ -313,15 +315,16 @@ def paged_attention(out, q, k_pages, v_pages, page_table, q_start, kv_lens, *, s
     paged_attention_workspace_bytes, 256-byte aligned, not shared by overlapping calls; None takes one from torch."""
     kv, device, heads, d, code = _paged_kv(k_pages, v_pages, page_table, q_start, kv_lens)
     n = q.shape[0]
-    width = q.shape[1] * (q.shape[2] if q.dim() == 3 else 1)
+    width = _width(q)
     qp, q_stride = _rows(q, "q", k_pages.dtype, device, n, width)
     op, o_stride = _rows(out, "out", k_pages.dtype, device, n, width)
     if width % d:
         raise ValueError("q: expected whole heads")
     if workspace is None:
         workspace = torch.empty(_workspace_bytes(device, n, width // d, heads, d, code), dtype=torch.uint8, device=k_pages.device)
+    size = workspace.numel()
     desc = _ATTN.pack(op, o_stride, qp, q_stride, n, width // d, scale, window, max_new, max_len,
-                      _tensor(workspace, "workspace", torch.uint8, device, 1), workspace.shape[0])
+                      _vector(workspace, "workspace", torch.uint8, device, size), size)
     _on(device, _lib.mf_paged_attention, kv, desc)
 
 
