@@ -147,17 +147,19 @@ enum SbMode { SB_COUNT, SB_WEIGHT };
 // operations of exp(); rows that keep most of the vocabulary spend their time here.
 struct SbTemp {
     double inv_t, inv_step;  // 1 / T, 256 / (T ln 2)
+    float inv_f;
 };
 MF_DEVICE SbTemp sb_temp(double t) {
     SbTemp s;
     s.inv_t = 1.0 / t;
     s.inv_step = 369.3299304675746 * s.inv_t;  // 256 / ln 2
+    s.inv_f = (float)s.inv_t;
     return s;
 }
 MF_DEVICE u64 sb_weight(float x, float top, const SbTemp& s, const double* table) {
     if (x == top) return (u64)SB_ONE;
+    if (!((top - x) * s.inv_f < 32.25f)) return 0;  // below half of 2^-45 (with room for the float's error)
     const double z = (double)top - (double)x, e = z * s.inv_t;
-    if (!(e < 32.0)) return 0;  // below half of 2^-45
     const double magic = 6755399441055744.0;  // 1.5 * 2^52: the low bits of the sum are a whole number
     const double kk = fma(z, s.inv_step, magic);
     const int n = __double2loint(kk);
@@ -262,32 +264,49 @@ MF_DEVICE void sb_note(SbShared* sh, uint32_t key, uint32_t idx) {
     if (at < SB_FEW) sh->cand[at] = (u64)key << 32 | (uint32_t)~idx;
 }
 
-// Walks the block's slice and hands the values that `take` accepts to `add`, a
-// full warp of them at a time: few of many are accepted, and `add` is dear.
-template <typename Take, typename Add> MF_DEVICE void sb_scan_slice(const SbRow& r, Take take, Add add) {
+// Walks the block's slice: `note` gets every value between lo and hi (both
+// included) with its index, `add` every value above hi, a full warp of them at
+// a time: few of many are above, and `add` is dear. Four values per load.
+template <typename Note, typename Add> MF_DEVICE void sb_scan_slice(const SbRow& r, float lo, float hi, Note note, Add add) {
     const int lane = threadIdx.x & 31;
     float* queue = r.sh->queue[threadIdx.x >> 5];
     int n = 0;
-    for (int i0 = threadIdx.x & ~31; i0 < r.n; i0 += SB_THREADS) {
+    auto drain = [&] {  // the last 32
+        __syncwarp();
+        const int k = min(n, 32);
+        if (lane < k) add(queue[n - k + lane]);
+        n -= k;
+        __syncwarp();
+    };
+    const int n4 = r.n / 4;
+    for (int i0 = threadIdx.x & ~31; i0 < n4; i0 += SB_THREADS) {
         const int i = i0 + lane;
-        const float x = i < r.n ? r.vals[i] : 0.f;
-        const bool yes = i < r.n && take(x, i);
-        const unsigned who = __ballot_sync(0xffffffffu, yes);
-        if (yes) queue[n + __popc(who & ((1u << lane) - 1))] = x;
-        n += __popc(who);
-        if (n >= 32) {
-            __syncwarp();
-            add(queue[lane]);
-            __syncwarp();
-            n -= 32;
-            const float left = queue[32 + lane];
-            __syncwarp();
-            if (lane < n) queue[lane] = left;
+        const float4 v = i < n4 ? *reinterpret_cast<const float4*>(r.vals + 4 * i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        const bool in = i < n4;
+        if (!__any_sync(0xffffffffu, in && fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= lo)) continue;
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool above = in && x[e] > hi;
+            const unsigned who = __ballot_sync(0xffffffffu, above);
+            if (above) queue[n + __popc(who & ((1u << lane) - 1))] = x[e];
+            n += __popc(who);
+            if (in && !above && x[e] >= lo) note(x[e], r.base + 4 * i + e);
+            if (n >= 32) drain();
         }
     }
-    __syncwarp();
-    if (lane < n) add(queue[lane]);
-    __syncwarp();
+    // the last values of a slice that is no multiple of four
+    {
+        const int i = 4 * n4 + (int)threadIdx.x;
+        const bool in = i < r.n;
+        const float x = in ? r.vals[i] : 0.f;
+        const bool above = in && x > hi;
+        const unsigned who = __ballot_sync(0xffffffffu, above);
+        if (above) queue[n + __popc(who & ((1u << lane) - 1))] = x;
+        n += __popc(who);
+        if (in && !above && x >= lo) note(x, r.base + i);
+    }
+    while (n > 0) drain();
 }
 
 // Number of noted candidates of each block and of all. The blocks are in step before.
@@ -752,25 +771,28 @@ __global__ void __launch_bounds__(SB_THREADS, 2) sample_batch_kernel(const Sampl
             u64 s = 0;
             const float low_x = low ? sb_value(low) : -INFINITY;
             const bool same = temp == 1.f && !low;  // both borders have the same weights: one set of bins
-            if (cut_p) {
-#pragma unroll 2
-                for (int i = tid; i < r.n; i += SB_THREADS) {
-                    const float x = sb_vals[i];
-                    const int bin = sb_bin(r.top, x);
+            auto one = [&](float x) {
+                const int bin = sb_bin(r.top, x);
+                if (cut_p) {
                     s += sb_weight(x, r.top, t1, sh.table);
                     atomicAdd(&sh.part[0][bin], sb_coarse(r.top, x, bin, c1));
-                    if (!same && x >= low_x) atomicAdd(&sh.part[1][bin], sb_coarse(r.top, x, bin, c2));
-                }
-            } else {
-#pragma unroll 2
-                for (int i = tid; i < r.n; i += SB_THREADS) {
-                    const float x = sb_vals[i];
-                    if (!(x >= low_x)) continue;
-                    const int bin = sb_bin(r.top, x);
+                    if (same || !(x >= low_x)) return;
+                } else {
                     s += sb_weight(x, r.top, t2, sh.table);
-                    atomicAdd(&sh.part[1][bin], sb_coarse(r.top, x, bin, c2));
                 }
+                atomicAdd(&sh.part[1][bin], sb_coarse(r.top, x, bin, c2));
+            };
+            const float least = cut_p ? -INFINITY : low_x;  // what counts for the sum
+            const int n4 = r.n / 4;
+            for (int i = tid; i < n4; i += SB_THREADS) {
+                const float4 x = *reinterpret_cast<const float4*>(sb_vals + 4 * i);
+                if (x.x >= least) one(x.x);
+                if (x.y >= least) one(x.y);
+                if (x.z >= least) one(x.z);
+                if (x.w >= least) one(x.w);
             }
+            for (int i = 4 * n4 + tid; i < r.n; i += SB_THREADS)
+                if (sb_vals[i] >= least) one(sb_vals[i]);
             u64 block;
             sb_scan(s, &sh, block);
             if (tid == 0) sh.sum[0] = block;
@@ -789,15 +811,19 @@ __global__ void __launch_bounds__(SB_THREADS, 2) sample_batch_kernel(const Sampl
                 const int bin = sb_first_thread(w1 > 0 && (double)w1 >= share_p * (double)all1, &sh);
                 u64 s1 = 0, s2 = 0;
                 const bool same_t = temp == 1.f;
-                sb_scan_slice(r, [&](float x, int i) {
-                    const int b = sb_bin(r.top, x);
-                    if (b == bin) sb_note(&sh, sb_key(x), r.base + i);
-                    return b < bin;
-                }, [&](float x) {
+                // values above `hi` are certainly in a bin before, those below `lo` in one behind
+                const float hi = bin > 0 ? __fsub_ru(r.top, ((float)bin - 0.51f) / 16.f) : INFINITY;
+                const float lo = bin < SB_BINS - 1 ? __fsub_rd(r.top, ((float)bin + 0.51f) / 16.f) : -INFINITY;
+                auto before = [&](float x) {
                     const u64 w = sb_weight(x, r.top, t1, sh.table);
                     s1 += w;
                     if (x >= low_x) s2 += same_t ? w : sb_weight(x, r.top, t2, sh.table);
-                });
+                };
+                sb_scan_slice(r, lo, hi, [&](float x, int i) {
+                    const int b = sb_bin(r.top, x);
+                    if (b == bin) sb_note(&sh, sb_key(x), i);
+                    else if (b < bin) before(x);
+                }, before);
                 u64 b1, b2;
                 sb_scan(s1, &sh, b1);
                 sb_scan(s2, &sh, b2);
@@ -858,12 +884,16 @@ __global__ void __launch_bounds__(SB_THREADS, 2) sample_batch_kernel(const Sampl
                 const int bin = min(sb_first_thread(w2 > 0 && (double)w2 >= draw * (double)sum, &sh), last);
                 u64 s2 = 0;
                 const float kept_x = kept.key ? sb_value(kept.key) : -INFINITY;
-                sb_scan_slice(r, [&](float x, int i) {
-                    if (!(x >= low_x) || x < kept_x || (x == kept_x && (uint32_t)(r.base + i) > kept.idx)) return false;
+                // as above; what the filters cut is between (values below low_x or the last kept are never above `hi`)
+                const float hi = fmaxf(bin > 0 ? __fsub_ru(r.top, ((float)bin - 0.51f) / 16.f) : INFINITY, fmaxf(kept_x, low_x));
+                const float lo = bin < SB_BINS - 1 ? __fsub_rd(r.top, ((float)bin + 0.51f) / 16.f) : -INFINITY;
+                auto before = [&](float x) { s2 += sb_weight(x, r.top, t2, sh.table); };
+                sb_scan_slice(r, lo, hi, [&](float x, int i) {
+                    if (!(x >= low_x) || x < kept_x || (x == kept_x && (uint32_t)i > kept.idx)) return;
                     const int b = sb_bin(r.top, x);
-                    if (b == bin) sb_note(&sh, sb_key(x), r.base + i);
-                    return b < bin;
-                }, [&](float x) { s2 += sb_weight(x, r.top, t2, sh.table); });
+                    if (b == bin) sb_note(&sh, sb_key(x), i);
+                    else if (b < bin) before(x);
+                }, before);
                 u64 b2;
                 sb_scan(s2, &sh, b2);
                 if (tid == 0) sh.sum[0] = b2;
