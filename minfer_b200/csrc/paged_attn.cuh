@@ -14,7 +14,10 @@
 //   is not what bounds it; their sums are added at the end of an item.
 // Tiles are stored without padding, 16-byte pieces c of row r at c ^ (r & 7)
 // (no bank conflicts in either direction), so that two CTAs fit an SM and one
-// computes while the other's softmax waits at a barrier.
+// computes while the other's softmax waits at a barrier (298 -> 217 us for
+// chunks of 65 and single tokens over 4096 keys, 16/8 heads; 206 with items of
+// nearly equal rows). Bound by instruction issue: about a quarter of the FMA
+// rate in useful products, the rest are loads, exponentials and unused rows.
 #pragma once
 
 #include "paged_work.cuh"

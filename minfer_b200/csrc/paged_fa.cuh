@@ -17,7 +17,7 @@
 //                   from TMEM, B = V as it lies in the page: the key rows are
 //                   the K extent, d is contiguous).
 //   warps 9, 10     bring in K and V: one TMA box per run of R keys of a page
-//                   (R = the power of two in page_size, 8 .. 128). Runs that no
+//                   (R = the power of two in page_size, 8 .. 64). Runs that no
 //                   row sees or that have no page are not read: their scores
 //                   are masked, their V rows zeroed, so nothing in them (NaN
 //                   included) reaches a result; a run that is seen in part is
@@ -27,9 +27,16 @@
 // may overwrite P_i once O_i += P_i V has been issued, and a thread that sees
 // the commit of S_i knows that O_i holds every tile before.
 //
-// Bound by the exponentials as much as by the tensor core: 128 x 128 scores
-// cost 1024 cycles of the special-function unit and, at D = 128, 1024 of the
-// tensor core.
+// At D = 128 a pair of 128 x 128 score tiles costs 2048 cycles of the tensor
+// core and as many of the special-function unit (1536 with a quarter of the
+// exponentials on the FMA units). A tile's softmax (2200 cycles) and its MMAs
+// with their barriers (1200) follow each other, so a pair takes about 3450.
+// Measured: 4096 x 4096 causal, 32/8 heads, 142-162 us (0.52-0.59 of the cuBLAS
+// bf16 rate, diagonal tiles counted by their halves); 512 tokens after 28672,
+// 64/8 heads, 451-472 us (1.03-1.08 PFLOP/s on the 128 SMs that have a tile).
+// Slower: two buffers of 64-key scores (159 / 513 us: an MMA of 64 keys takes
+// 55 cycles, not 32), four groups of 64 columns (158 / 444), exponentials before
+// the maximum is known (154 / 470).
 #pragma once
 
 #include <type_traits>

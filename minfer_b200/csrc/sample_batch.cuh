@@ -12,16 +12,29 @@
 // target.
 //
 // A row lives in the shared memory of one thread-block cluster: the logits are
-// read from memory once, and every later pass runs on chip. A border is found by descent: 512 bins of 1/16 below the top,
-// the bin that holds the border cut into 512 ranges of keys, and so on, until
-// a few candidates are left, which one warp orders, or one value, whose ties
-// are counted out by index. Per level the bins of the cluster's blocks are
-// added up by every block for itself (one remote read per block and bin).
+// read from memory once, and every later pass runs on chip.
+//   top_k: the threads' maxima bound the k-th candidate; what is above goes to
+//   the row's first block, which finds every border among it (sb_pick).
+//   Otherwise: one pass adds up the exact weights and, coarsely, 512 bins of
+//   1/16 below the top, which tell the border's bin; another adds up exactly
+//   what lies before that bin and sends the bin to the first block.
+//   Where a bin holds too many candidates, or the coarse sums named the wrong
+//   one (the exact sums tell): by descent over the cluster (sb_find), the bin
+//   that holds the border cut into 512 ranges of keys, and so on, until a few
+//   candidates are left, or one value, whose ties are counted out by index.
 //
 // Sums: weights are exp() in 64 bits, rounded to multiples of 2^-45 and added
 // as whole numbers, so a sum does not depend on the order of its terms and is
 // off by at most 2^-46 per term. In floats a vocabulary of 10^5 would move the
 // border of every hundredth draw.
+//
+// Measured, 151936 fp32 logits: one row 15 us with top_k 50, 46 with top_p 0.9
+// alone; 64 rows 41 and 125 us (the floor, one read, is 6; the maximum alone
+// takes 13). Bound by latencies (an exchange over the cluster is about a
+// microsecond, and there are five to nine) and, without top_k, by shared-memory
+// atomics and 64-bit arithmetic. Exact bins took three atomics per logit more
+// (147 us for a mixed batch of 64 rows, now 79), a bitonic sort of the
+// candidates 14 us more per border.
 #pragma once
 
 #include "mf_common.cuh"
