@@ -57,10 +57,6 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 3) paged_rope_kernel(const Pa
     const long long unit = (long long)blockIdx.x * ROPE_WARPS + (threadIdx.x >> 5);
     const int t = (int)(unit / chunks);
     if (t >= p.n_tokens) return;
-    const int b = paged_owner(p, t);
-    if (b < 0) return;  // rows behind the last sequence stay as they are
-    const PagedSeq s = paged_seq(p, b);
-    const int pos = s.first + (t - s.row);
     const int h0 = (int)(unit % chunks) * r.hpw, h1 = min(h0 + r.hpw, H);
 
     // the blocks of this lane (4 elements each)
@@ -72,6 +68,24 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 3) paged_rope_kernel(const Pa
         blk[u][0] = i < hb ? i : 2 * hb + 2 * (i - hb);
         blk[u][1] = i < hb ? i + hb : blk[u][0] + 1;
     }
+    // Four heads at a time; the next four are on their way while these are turned, the first while the token's
+    // sequence, page and angles are found.
+    const X* x0 = reinterpret_cast<const X*>(r.qkv) + t * r.x_stride;
+    PackV<X, 4> next[NS][2];
+    auto fetch = [&](int h) {
+        if (h < h1) {
+#pragma unroll
+            for (int u = 0; u < NS; ++u)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) next[u][w] = *reinterpret_cast<const PackV<X, 4>*>(x0 + (long long)h * D + 4 * blk[u][w]);
+        }
+    };
+    fetch(h0 + sub);
+    const int b = paged_owner(p, t);
+    if (b < 0) return;  // rows behind the last sequence stay as they are
+    const PagedSeq s = paged_seq(p, b);
+    const int pos = s.first + (t - s.row);
+
     // cos and sin of this lane's pairs (1 and 0 behind d_rot); the four heads' lanes share the work
     float c[NA], sn[NA];
     if (h0 < Hq + Hk) {
@@ -99,83 +113,72 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 3) paged_rope_kernel(const Pa
     }
     const int page = paged_page(p, b, pos);
     const long long kv_row = page >= 0 ? page * p.page_stride + (long long)(pos % p.page_size) * p.row_stride : 0;
-    const X* x0 = reinterpret_cast<const X*>(r.qkv) + t * r.x_stride;
 
-    constexpr int HB = 2;  // rounds of four heads in flight
-    for (int hg = h0; hg < h1; hg += HB * ROPE_HEADS) {
-        PackV<X, 4> in[HB][NS][2];
+    for (int hg = h0; hg < h1; hg += ROPE_HEADS) {
+        const int h = hg + sub;
+        PackV<X, 4> in[NS][2];
 #pragma unroll
-        for (int v = 0; v < HB; ++v) {
-            const int h = hg + ROPE_HEADS * v + sub;
-            if (h < h1) {
+        for (int u = 0; u < NS; ++u)
 #pragma unroll
-                for (int u = 0; u < NS; ++u)
+            for (int w = 0; w < 2; ++w) in[u][w] = next[u][w];
+        fetch(h + ROPE_HEADS);
+        const bool live = h < h1, is_q = h < Hq, is_v = h >= Hq + Hk;
+        float x[NS][2][4];
 #pragma unroll
-                    for (int w = 0; w < 2; ++w) in[v][u][w] = *reinterpret_cast<const PackV<X, 4>*>(x0 + (long long)h * D + 4 * blk[u][w]);
-            }
-        }
+        for (int u = 0; u < NS; ++u)
 #pragma unroll
-        for (int v = 0; v < HB; ++v) {
-            const int h = hg + ROPE_HEADS * v + sub;
-            if (hg + ROPE_HEADS * v >= h1) break;  // the whole warp
-            const bool live = h < h1, is_q = h < Hq, is_v = h >= Hq + Hk;
-            float x[NS][2][4];
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[u][w][e] = live ? to_f<X>(in[u][w].e[e]) : 0.f;
+        const float* nw = is_q ? r.q_norm_w : r.k_norm_w;
+        if ((r.q_norm_w || r.k_norm_w) && hg < Hq + Hk) {  // the whole warp
+            float ss = 0.f;
 #pragma unroll
             for (int u = 0; u < NS; ++u)
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[u][w][e] = live ? to_f<X>(in[v][u][w].e[e]) : 0.f;
-            const float* nw = is_q ? r.q_norm_w : r.k_norm_w;
-            if ((r.q_norm_w || r.k_norm_w) && hg + ROPE_HEADS * v < Hq + Hk) {  // the whole warp
-                float ss = 0.f;
+                    for (int e = 0; e < 4; ++e) ss = fmaf(x[u][w][e], x[u][w][e], ss);
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (nw && !is_v) {
+                const float inv = rsqrtf(ss / (float)D + r.eps);
 #pragma unroll
                 for (int u = 0; u < NS; ++u)
 #pragma unroll
                     for (int w = 0; w < 2; ++w)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) ss = fmaf(x[u][w][e], x[u][w][e], ss);
-#pragma unroll
-                for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                if (nw && !is_v) {
-                    const float inv = rsqrtf(ss / (float)D + r.eps);
-#pragma unroll
-                    for (int u = 0; u < NS; ++u)
-#pragma unroll
-                        for (int w = 0; w < 2; ++w)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) x[u][w][e] = x[u][w][e] * inv * __ldg(nw + 4 * blk[u][w] + e);
-                }
+                        for (int e = 0; e < 4; ++e) x[u][w][e] = x[u][w][e] * inv * __ldg(nw + 4 * blk[u][w] + e);
             }
-            if (!is_v) {
-#pragma unroll
-                for (int u = 0; u < NS; ++u) {
-                    if (l + 8 * u >= hb) continue;  // behind d_rot: as it is
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        auto turn = [&](float& a, float& z) {
-                            const float xa = a, xz = z;
-                            a = fmaf(xa, c[4 * u + e], -xz * sn[4 * u + e]);
-                            z = fmaf(xz, c[4 * u + e], xa * sn[4 * u + e]);
-                        };
-                        if (r.interleaved) turn(x[u][e >> 1][2 * (e & 1)], x[u][e >> 1][2 * (e & 1) + 1]);
-                        else turn(x[u][0][e], x[u][1][e]);
-                    }
-                }
-            }
-            if (!live || (!is_q && page < 0)) continue;
-            T* dst = is_q ? reinterpret_cast<T*>(r.q_out) + t * r.q_stride + (long long)h * D
-                          : reinterpret_cast<T*>(is_v ? p.v : p.k) + kv_row + (long long)(h - Hq - (is_v ? Hk : 0)) * p.head_stride;
-#pragma unroll
-            for (int u = 0; u < NS; ++u)
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    PackV<T, 4> y;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y.e[e] = from_f<T>(x[u][w][e]);
-                    *reinterpret_cast<PackV<T, 4>*>(dst + 4 * blk[u][w]) = y;
-                }
         }
+        if (!is_v) {
+#pragma unroll
+            for (int u = 0; u < NS; ++u) {
+                if (l + 8 * u >= hb) continue;  // behind d_rot: as it is
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    auto turn = [&](float& a, float& z) {
+                        const float xa = a, xz = z;
+                        a = fmaf(xa, c[4 * u + e], -xz * sn[4 * u + e]);
+                        z = fmaf(xz, c[4 * u + e], xa * sn[4 * u + e]);
+                    };
+                    if (r.interleaved) turn(x[u][e >> 1][2 * (e & 1)], x[u][e >> 1][2 * (e & 1) + 1]);
+                    else turn(x[u][0][e], x[u][1][e]);
+                }
+            }
+        }
+        if (!live || (!is_q && page < 0)) continue;
+        T* dst = is_q ? reinterpret_cast<T*>(r.q_out) + t * r.q_stride + (long long)h * D
+                      : reinterpret_cast<T*>(is_v ? p.v : p.k) + kv_row + (long long)(h - Hq - (is_v ? Hk : 0)) * p.head_stride;
+#pragma unroll
+        for (int u = 0; u < NS; ++u)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                PackV<T, 4> y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y.e[e] = from_f<T>(x[u][w][e]);
+                *reinterpret_cast<PackV<T, 4>*>(dst + 4 * blk[u][w]) = y;
+            }
     }
 }
 
