@@ -341,11 +341,22 @@ static int rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* d, void*
     r.n_heads = d->n_heads;
     r.d_rot = d->d_rot;
     r.interleaved = d->interleaved != 0;
-    // Heads per warp: the angles cost about as much as eight heads, so a warp
-    // takes more than its four at a time as soon as the warps still fill the SMs.
+    // Heads per warp, in fours: a warp's angles and lookups take as long as about
+    // eight heads, and blocks run in whole rounds (three blocks per SM), so the
+    // number with the shortest rounds x (heads + 8) is taken. (2533 tokens of 80
+    // heads: 20 heads, 3 rounds, 29 us; 32 heads, 3 rounds of which the last is a
+    // seventh full, 33 us. One token: 4 heads.)
     const int H = d->n_heads + 2 * kv->n_kv_heads;
-    const long long warps = (long long)num_sms() * 32;
-    r.hpw = (int)std::min<long long>(std::max<long long>((long long)d->n_tokens * H / warps / 4 * 4, 4), 32);
+    const long long resident_warps = 3ll * num_sms() * mf::ROPE_WARPS;
+    long long least = 0;
+    for (int n = 4; n == 4 || (n <= 64 && n < H + 4); n += 4) {
+        const long long warps = (long long)d->n_tokens * ((H + n - 1) / n);
+        const long long cost = (warps + resident_warps - 1) / resident_warps * (n + 8);
+        if (n == 4 || cost < least) {
+            least = cost;
+            r.hpw = n;
+        }
+    }
     const long long units = (long long)d->n_tokens * ((H + r.hpw - 1) / r.hpw);
     const long long blocks = (units + mf::ROPE_WARPS - 1) / mf::ROPE_WARPS;
     if (blocks > 0x7fffffffll) return fail(MF_E_UNSUPPORTED, "too many rows");

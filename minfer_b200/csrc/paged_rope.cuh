@@ -20,8 +20,8 @@
 // by two; so rotating needs no exchange, and the norm three shuffles for four
 // heads. (With a head across the warp the sums and exchanges took 90
 // instructions a head, more time than its 768 bytes: 42 us for the chunk below.)
-// Measured: 156 MB (fp32 rows of 80 heads to bf16) in 34 us, 0.70 of the copy
-// rate; 33 with a 64-register limit (but 4.6 us instead of 3.7 for 64 tokens).
+// Measured: 156 MB (fp32 rows of 80 heads to bf16) in 29 us on inputs that are
+// partly in L2, 31 on new ones (0.76 of the copy rate); one token 3.2 us.
 #pragma once
 
 #include "paged.cuh"
