@@ -191,7 +191,8 @@ template <int RT, int KT> MF_DEVICE void paged_next(const PagedKv& p, const Page
 // Joins the parts of every item that a cut divides: block c - 1 takes the item
 // whose first inner cut is c (1 .. grid - 1). Row by row, with m the largest
 // part maximum, out = sum O_i 2^(m_i - m) / sum l_i 2^(m_i - m). A part that
-// saw no key has m = -inf and adds nothing; a row without any key is 0.
+// saw no key has l = 0 and adds nothing; a row without any key is 0. A part
+// whose scores were NaN has l = NaN, whatever its m, and makes the row NaN.
 // The search for the item runs before the wait for the kernel that leaves the
 // parts: that kernel lets this one start only after its own wait, so the
 // batch's lengths are there.
@@ -219,13 +220,14 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedKv p, const 
         float m = -INFINITY;
         for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(ml + ((long long)(2 * (c - 1 + i) + (i == 0)) * RT + r) * 2));
         m = warp_max(m);
+        if (m == -INFINITY) m = 0.f;
         float l = 0.f, o[V] = {};
-        for (int i0 = 0; i0 < n && m != -INFINITY; i0 += 32) {
+        for (int i0 = 0; i0 < n; i0 += 32) {
             float w = 0.f;  // weight of part i0 + lane
             if (i0 + lane < n) {
                 const int i = i0 + lane;
                 const float2 v = __ldcg(reinterpret_cast<const float2*>(ml) + (long long)(2 * (c - 1 + i) + (i == 0)) * RT + r);
-                w = v.x == -INFINITY ? 0.f : exp2f(v.x - m);
+                w = v.y == 0.f ? 0.f : exp2f(v.x - m);
                 l = fmaf(v.y, w, l);
             }
             for (int i1 = 0; i1 < min(32, n - i0); i1 += U) {  // U loads in flight
