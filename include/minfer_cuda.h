@@ -519,7 +519,9 @@ int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* desc, 
  * to pos) of scale * q.k_s, times v_s; query heads share KV head h / G. A row
  * that sees no position is 0. Positions that no row of the call sees are never
  * used, whatever their pages hold; a position that some rows of a sequence see
- * must hold finite values (it may enter the others' sums with weight 0).
+ * must hold finite values (it may enter the others' sums with weight 0). A row
+ * with a score of NaN or +inf is NaN; scores of -inf weigh nothing, alone they
+ * leave the row 0.
  * max_new and max_len (0: unknown) are hints, the largest n_b and kv_lens[b]:
  * they choose between kernels, never what is computed. The workspace
  * (mf_paged_attention_workspace_bytes, 256-byte aligned) needs no

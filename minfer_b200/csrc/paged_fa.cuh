@@ -131,14 +131,20 @@ MF_DEVICE f32x2 pf_add2(f32x2 a, f32x2 b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// Maxima that are NaN where an argument is.
 MF_DEVICE float pf_max3(float a, float b, float c) {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+MF_DEVICE float pf_max(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 // 2^y of two finite y on the FMA units: y = n + r, |r| <= 1/2, a polynomial of
 // degree 5 for 2^r (minimax, relative error 2^-23.6), n added to its exponent.
-// Below 2^-126 the result is a tiny number instead of zero.
+// Below 2^-126 the result is a tiny number instead of zero, and NaN is lost.
 MF_DEVICE float2 pf_exp2_fma(f32x2 y) {
     const float2 c = pf_each(y);
     y = pf_two(fmaxf(c.x, -126.f), fmaxf(c.y, -126.f));
@@ -450,10 +456,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 #pragma unroll
                     for (int u = 0; u < 4; ++u) m4[u] = pf_max3(m4[u], __uint_as_float(sr[c + u]), __uint_as_float(sr[c + 4 + u]));
 #pragma unroll
-                for (int u = 0; u < 4; ++u) m4[u] = fmaxf(m4[u], __uint_as_float(sr[124 + u]));
-                const float mx = fmaxf(pf_max3(m4[0], m4[1], m4[2]), m4[3]) * c2;
-                const bool bump = mx > m + 8.f;  // also the first keys of a row (m = -inf)
-                const float mu = bump ? mx : m;
+                for (int u = 0; u < 4; ++u) m4[u] = pf_max(m4[u], __uint_as_float(sr[124 + u]));
+                const float mx = pf_max(pf_max3(m4[0], m4[1], m4[2]), m4[3]) * c2;
+                // Also the first keys of a row (m = -inf), and a NaN or infinite score: m is then NaN (inf - inf), and with
+                // it every exponential of the special-function unit and the sum. The FMA units' alone would hide a NaN.
+                const bool bump = !(mx <= m + 8.f);
+                const float mu = bump ? mx + (mx - mx) : m;
                 const float base = mu == -INFINITY ? 0.f : mu;
                 const float alpha = bump ? ex2_approx(m - base) : 1.f;
                 m = mu;
@@ -506,7 +514,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                     mbar_arrive(&p_full[i][half]);
                 }
                 const float2 sum = pf_each(pf_add2(s2[0], s2[1]));
-                l = fmaf(l, alpha, sum.x + sum.y);
+                // scores that are all -inf add nothing (the FMA units make 2^-126 of them)
+                l = fmaf(l, alpha, mu == -INFINITY ? 0.f : sum.x + sum.y);
             }
             if (nt > 0) mbar_wait(&o_full[i], 0, deadline, failed);
             tc_fence_after();

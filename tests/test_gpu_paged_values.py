@@ -42,3 +42,51 @@ def test_nan_queries_stay_nan(dtype, seqs):
     out = run(b, q)
     assert out[bad].isnan().all()
     assert torch.equal(out[~bad], want[~bad])
+
+
+@TYPES
+@BATCHES
+@pytest.mark.parametrize("what", ["nan", "inf"])
+def test_nan_and_infinite_scores_show(dtype, seqs, what):
+    """One key whose score is NaN, or +inf (softmax of it is inf - inf), makes NaN of every row that sees it, at any
+    place of its group of keys."""
+    if what == "inf" and dtype == F16:
+        pytest.skip("no finite fp16 operands have an infinite score")
+    b = ref.Batch(seqs, 8, 2, 128, 16, dtype, seed=2)
+    q = b.q()
+    q[:, :, 3] = 9.0
+    want = run(b, q)
+    for at in range(8):
+        pages = [(b.table[s, 0], (at + s) % 8) for s in range(len(seqs))]
+        saved = [b.k[p, 0, r].clone() for p, r in pages]
+        for p, r in pages:
+            b.k[p, 0, r] = 0
+            b.k[p, 0, r, 3] = math.nan if what == "nan" else 3e38
+        out = run(b, q)
+        for s, (n, length) in enumerate(seqs):
+            sees = torch.arange(length - n, length, device="cuda") >= (at + s) % 8
+            rows = out[b.start[s]:b.start[s] + n, :4]
+            assert rows[sees].isnan().all() and torch.isfinite(rows[~sees]).all()
+        assert torch.equal(out[:, 4:], want[:, 4:])
+        for (p, r), x in zip(pages, saved):
+            b.k[p, 0, r] = x
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@BATCHES
+def test_scores_of_minus_infinity_weigh_nothing(dtype, seqs):
+    """Scores that overflow to -inf are as if masked: alone they leave a row 0, beside others they add nothing."""
+    b = ref.Batch(seqs, 8, 2, 128, 16, dtype, seed=3)
+    q = torch.full((b.total, 8, 128), 1e20, dtype=dtype, device="cuda")
+    keys = [(b.table[s, i // 16], i % 16) for s in range(len(seqs)) for i in range(seqs[s][1])]
+    pages, rows = (torch.tensor(x, device="cuda") for x in zip(*[(int(p), r) for p, r in keys]))
+    b.k[pages, :, rows] = torch.full((), -1e20, dtype=dtype, device="cuda")
+    assert (run(b, q) == 0).all()
+    for s in range(len(seqs)):  # one key of each sequence that counts
+        b.k[b.table[s, 0], :, 2] = 0
+    out = run(b, q)
+    for s, (n, length) in enumerate(seqs):
+        v = b.v[b.table[s, 0], :, 2].repeat_interleave(4, 0)
+        sees = torch.arange(length - n, length, device="cuda") >= 2
+        rows = out[b.start[s]:b.start[s] + n]
+        assert torch.equal(rows[sees], v.expand_as(rows)[sees]) and (rows[~sees] == 0).all()
