@@ -544,8 +544,8 @@ typedef struct mf_paged_attn_desc {
 size_t mf_paged_attention_workspace_bytes(int n_tokens, int n_heads, int n_kv_heads, int d_head, int dtype);
 int mf_paged_attention(const mf_paged_kv* kv, const mf_paged_attn_desc* desc, void* stream);
 /* Status bits of the paged attention kernels since the last clear (2: a wait
- * gave up, after MF_PREFILL_TIMEOUT_MS, default 2000; its outputs are then not
- * written). Synchronises the device. */
+ * gave up, after MF_PREFILL_TIMEOUT_MS, default 2000; the rows of out that were
+ * not finished are then as they were). Synchronises the device. */
 int mf_paged_status(int* status, int clear);
 
 /* ===================================================================== */

@@ -437,6 +437,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                 const int c0 = k0 + 8 * (lane & 15);
                 const unsigned ok = __ballot_sync(0xffffffffu, c0 < span.hi && paged_page(p, pt.b, c0) >= 0) & 0xffffu;
                 mbar_wait(&s_full[i], (uint32_t)j & 1u, deadline, failed);
+                failed = __any_sync(0xffffffffu, failed);
+                if (failed) break;  // without an arrival: no product of a tile whose P is not there
                 tc_fence_after();
                 uint32_t sr[128];
 #pragma unroll
@@ -523,7 +525,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             const long long orow = (long long)(s.row + tok) * a.n_heads + h * a.G + g;
             const long long prow = (long long)blockIdx.y * p.n_tokens * a.n_heads + orow;
             T* out = reinterpret_cast<T*>(a.out) + (long long)(s.row + tok) * a.out_stride + (long long)(h * a.G + g) * D;
-            if (f.n_split > 1 && live && !failed) f.part_ml[prow] = make_float2(m, l);
+            if (f.n_split > 1 && live) f.part_ml[prow] = failed ? make_float2(0.f, PAGED_GAVE_UP) : make_float2(m, l);
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
@@ -577,6 +579,7 @@ __global__ void __launch_bounds__(256) paged_fa_join_kernel(const PagedKv p, con
     if (b < 0 || paged_seq(p, b).n * a.G <= f.min_rows) return;
     float2 ml = make_float2(-INFINITY, 0.f);
     if (lane < f.n_split) ml = __ldcg(f.part_ml + (long long)lane * rows + orow);
+    if (__any_sync(0xffffffffu, ml.y == PAGED_GAVE_UP)) return;
     const float m = warp_max(ml.x);
     const float w_mine = ml.y != 0.f ? exp2f(ml.x - m) : 0.f;  // NaN stays
     const float l = warp_sum(ml.y * w_mine);

@@ -199,6 +199,8 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
             for (int j = j0; j < j1; ++j, ++n) {
                 const int st = n % ST;
                 mbar_wait(&full[st], (uint32_t)(n / ST) & 1u, deadline, failed);
+                failed = __any_sync(0xffffffffu, failed);
+                if (failed) break;  // without an arrival: the producer refills nothing that another warp still reads
                 const uint32_t kd = smem_u32(smem + st * 2 * TILE), vd = kd + TILE;
                 const int kw = KW * warp, k0 = key0 + j * KT + kw;  // this warp's keys
                 float s[MT][KW / 8][4];
@@ -334,12 +336,13 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                 for (int e = 0; e < 2; ++e) {
                     l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 1);
                     l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
-                    if ((lane & 3) == 0) ml_s[warp * RT + 16 * mt + 8 * e + (lane >> 2)] = make_float2(m[mt][e], l[mt][e]);
+                    if ((lane & 3) == 0) ml_s[warp * RT + 16 * mt + 8 * e + (lane >> 2)] = make_float2(m[mt][e], failed ? PAGED_GAVE_UP : l[mt][e]);
                 }
             const bool whole = j0 == 0 && j1 == it.tiles;
             const long long slot = 2ll * blockIdx.x + (j0 > 0 ? 0 : 1);
             float* part = a.part + slot * RT * D;
             float* part_ml = a.part + 2ll * gridDim.x * RT * D + slot * RT * 2;
+            bool stop = false;
 #pragma unroll
             for (int c0 = 0; c0 < D; c0 += PW_COLS) {
 #pragma unroll
@@ -363,13 +366,14 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                         const float2 y = ml_s[i * RT + r];
                         const float wt = y.y != 0.f ? ex2_approx(y.x - mm) : 0.f;
                         const float4 v = *reinterpret_cast<const float4*>(join + (i * RT + r) * PW_LD + c);
+                        stop |= y.y == PAGED_GAVE_UP;  // of every row, so all four warps know
                         ll = fmaf(y.y, wt, ll);
                         x.x = fmaf(v.x, wt, x.x);
                         x.y = fmaf(v.y, wt, x.y);
                         x.z = fmaf(v.z, wt, x.z);
                         x.w = fmaf(v.w, wt, x.w);
                     }
-                    if (r < rows && !failed) {
+                    if (r < rows && !stop) {
                         if (whole) {
                             const float inv = ll == 0.f ? 0.f : 1.0f / ll;
                             T* out = reinterpret_cast<T*>(a.out) + (long long)(it.s.row + (it.r0 + r) / a.G) * a.out_stride +
@@ -382,6 +386,12 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                     }
                 }
                 named_bar_sync(1, PW_WARPS * 32);
+            }
+            if (stop) {
+                // nothing of this item or the next ones is written, and neither are the divided ones joined
+                float2* ml = reinterpret_cast<float2*>(a.part + 2ll * gridDim.x * RT * D) + 2ll * blockIdx.x * RT;
+                if (threadIdx.x < 2 * RT) ml[threadIdx.x] = make_float2(0.f, PAGED_GAVE_UP);
+                break;
             }
             w = it.start + j1;
             if (w < w1) paged_next<RT, KT>(p, a, it);

@@ -28,10 +28,14 @@ struct PagedAttn {
     int n_heads, G, window;
     int min_rows, max_rows;  // sequences of other numbers of rows (n_b * G) are another kernel's: min_rows < rows <= max_rows
     int beside;    // launched behind a chunk kernel that it neither reads nor waits for at its start (paged_begin)
-    float* part;   // (O, m, l) of divided items: [2 * grid][RT][D], then [2 * grid][RT][2]
+    float* part;   // (O, m, l) of divided items: [2 * grid][RT][D], then [2 * grid][RT][2]; l = PAGED_GAVE_UP: none
     int* status;   // bit 2: a wait gave up
     unsigned long long timeout_ns;
 };
+
+// The sum that a CTA whose wait gave up leaves in place of its rows': the
+// joining kernels write no row with such a part. (Sums are not negative.)
+constexpr float PAGED_GAVE_UP = -1.f;
 
 // A kernel for few rows that follows a chunk kernel of the same call works on
 // other rows, so it starts as that kernel's CTAs leave the SMs and waits for it
@@ -222,11 +226,13 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedKv p, const 
         m = warp_max(m);
         if (m == -INFINITY) m = 0.f;
         float l = 0.f, o[V] = {};
+        bool gone = false;
         for (int i0 = 0; i0 < n; i0 += 32) {
             float w = 0.f;  // weight of part i0 + lane
             if (i0 + lane < n) {
                 const int i = i0 + lane;
                 const float2 v = __ldcg(reinterpret_cast<const float2*>(ml) + (long long)(2 * (c - 1 + i) + (i == 0)) * RT + r);
+                gone |= v.y == PAGED_GAVE_UP;
                 w = v.y == 0.f ? 0.f : exp2f(v.x - m);
                 l = fmaf(v.y, w, l);
             }
@@ -245,6 +251,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedKv p, const 
                 }
             }
         }
+        if (__any_sync(0xffffffffu, gone)) continue;
         l = warp_sum(l);
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         PackV<T, V> y;
