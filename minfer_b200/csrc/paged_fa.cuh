@@ -335,12 +335,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                 }
                 issued = j + 1;
             }
-            if (failed) {
-                // let the copies in flight land before shared memory goes away
-                bool f2 = false;
-                const unsigned long long d2 = globaltimer_ns() + a.timeout_ns;
-                for (int j = max(0, issued - PF_STAGES); j < issued; ++j) mbar_wait(&full[j % PF_STAGES], (uint32_t)(j / PF_STAGES) & 1u, d2, f2);
-            }
+            // the copies in flight land before shared memory goes away, also those that another warp gave up on
+            bool f2 = false;
+            const unsigned long long d2 = globaltimer_ns() + a.timeout_ns;
+            for (int j = max(0, issued - PF_STAGES); j < issued; ++j) mbar_wait(&full[j % PF_STAGES], (uint32_t)(j / PF_STAGES) & 1u, d2, f2);
         } else if (warp == 8 && nt > 0 && pf_elect()) {
             constexpr uint32_t idesc_s = fa_idesc(128, PF_KT, BF);
             constexpr uint32_t idesc_o = fa_idesc(128, D, BF) | (1u << 16);  // B's rows run along K
@@ -393,8 +391,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                 umma_commit(&v_free[j % PF_STAGES]);
                 if (more) umma_commit(&k_free[(j + 1) % PF_STAGES]);
             }
-            if (failed && any) {
-                // the MMAs already issued finish before TMEM is freed
+            if (any) {
+                // the MMAs already issued finish before TMEM is freed, also where the softmax gave up on the last ones
                 umma_commit(&drain);
                 bool f2 = false;
                 mbar_wait(&drain, 0, globaltimer_ns() + a.timeout_ns, f2);

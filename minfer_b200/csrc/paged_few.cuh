@@ -133,12 +133,10 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
             w = it.start + j1;
             if (w < w1 && !failed) paged_next<RT, KT>(p, a, it);
         }
-        if (failed) {
-            // let the copies in flight land before shared memory goes away
-            bool f2 = false;
-            const unsigned long long d2 = globaltimer_ns() + a.timeout_ns;
-            for (int j = max(0, n - ST); j < n; ++j) mbar_wait(&full[j % ST], (uint32_t)(j / ST) & 1u, d2, f2);
-        }
+        // the copies in flight land before shared memory goes away, also those that a consumer gave up on
+        bool f2 = false;
+        const unsigned long long d2 = globaltimer_ns() + a.timeout_ns;
+        for (int j = max(0, n - ST); j < n; ++j) mbar_wait(&full[j % ST], (uint32_t)(j / ST) & 1u, d2, f2);
     } else {
         const float c2 = fabsf(a.scale2);
         const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;  // a negative scale goes into Q's sign
