@@ -493,8 +493,9 @@ int mf_rope_freqs(double* out, int d_rot, double base, int scaling, double facto
  * module.cpp:193-226, src/ops/kernels.cpp:31-82): the rotated q heads go to
  * q_out, k and v to their page rows, rounded to the pages' type. The first
  * d_rot elements of a head are rotated in pairs (j, j + d_rot / 2), or
- * (2j, 2j + 1) with `interleaved`; the others pass through. Angles are reduced
- * in 64 bits, so far positions are as exact as near ones. */
+ * (2j, 2j + 1) with `interleaved`; the others pass through. Angles are the
+ * exact products of position and frequency, reduced and rounded once, so for
+ * the given frequencies far positions are as exact as near ones. */
 typedef struct mf_paged_rope_desc {
     void* q_out;        /* [n_tokens][q_stride], n_heads * d_head of each row */
     long long q_stride; /* elements; 0: n_heads * d_head */

@@ -8,10 +8,12 @@
 // the page of pos, in the cache's type.
 //
 // f_j is in turns per position and 64 bits: a float angle at position 10^6 is
-// off by up to 0.03 rad. pos * f_j is reduced to (-1/2, 1/2] turns in double
-// and only then rounded, so the angle's error is that of one float rounding
-// at every position. The two doubles per pair are computed once per token and
-// kept in registers over the warp's heads.
+// off by up to 0.03 rad. pos * f_j is reduced to about (-1/2, 1/2] turns in
+// double, with the product's own rounding error (up to 2^-25 turns at 2^31)
+// added back from a second product, and only then rounded: for a given f_j the
+// angle's error is that of one float rounding at every position. (f_j itself
+// is rounded to 64 bits, which at position p is p f_j 2^-53 turns.) The angles
+// are computed once per token and kept in registers over the warp's heads.
 //
 // Bound by memory: every value is read and written once. Eight lanes take a
 // head, a warp four heads at a time and `hpw` heads of one token in all. A lane
@@ -99,8 +101,9 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 3) paged_rope_kernel(const Pa
             if (i < hb) {
                 // half layout: (4 i + e, and half on); pairs: two of each block
                 const int j = !r.interleaved ? 4 * i + e : 2 * (e < 2 ? i : i + hb) + (e & 1);
-                const double turns = (double)(r.positions ? __ldg(r.positions + t) : pos) * __ldg(r.freqs + j);
-                sincospif(2.0f * (float)(turns - rint(turns)), &sv[v], &cv[v]);
+                const double at = r.positions ? __ldg(r.positions + t) : pos, f = __ldg(r.freqs + j);
+                const double turns = at * f, rest = fma(at, f, -turns);
+                sincospif(2.0f * (float)((turns - rint(turns)) + rest), &sv[v], &cv[v]);
                 cv[v] *= r.mscale;
                 sv[v] *= r.mscale;
             }
