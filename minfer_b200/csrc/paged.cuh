@@ -14,6 +14,8 @@
 
 #include "mf_common.cuh"
 
+#define MF_HOST_DEVICE __host__ __device__ __forceinline__  // counting that tests run on the CPU
+
 namespace mf {
 
 // Copy of mf_paged_kv with the strides resolved.

@@ -54,7 +54,7 @@ MF_DEVICE void paged_end(const PagedAttn& a) {
 struct PagedSpan {
     int lo, hi;
 };
-MF_DEVICE PagedSpan paged_span(const PagedSeq& s, const PagedAttn& a, int r0, int rows) {
+MF_HOST_DEVICE PagedSpan paged_span(const PagedSeq& s, const PagedAttn& a, int r0, int rows) {
     const int t0 = r0 / a.G, t1 = (min(r0 + rows, s.n * a.G) - 1) / a.G;
     PagedSpan k;
     k.hi = max(s.first + t1 + 1, 0);
@@ -62,21 +62,22 @@ MF_DEVICE PagedSpan paged_span(const PagedSeq& s, const PagedAttn& a, int r0, in
     return k;
 }
 // Number of KT-key tiles of a span; a span without keys still takes one (its rows' zeros are written).
-template <int KT> MF_DEVICE int paged_tiles(const PagedSpan& k) { return max((k.hi + KT - 1) / KT - k.lo / KT, 1); }
+template <int KT> MF_HOST_DEVICE int paged_tiles(const PagedSpan& k) { return max((k.hi + KT - 1) / KT - k.lo / KT, 1); }
 
 // Rows of an item of a sequence of `rows`: as few items as RT allows, of nearly
 // equal size (130 rows are three items of 48, not two of 64 and one of 2: a
 // warp works on 8 rows, and an item counts by its keys alone).
-template <int RT> MF_DEVICE int paged_step(int rows) {
+template <int RT> MF_HOST_DEVICE int paged_step(int rows) {
     const int n = (rows + RT - 1) / RT;
     return n <= 1 ? RT : min(((rows + n - 1) / n + 7) / 8 * 8, RT);
 }
 
-// Tiles of one KV head of sequence b (0: no rows, or another kernel's)
-template <int RT, int KT> MF_DEVICE int paged_head_work(const PagedSeq& s, const PagedAttn& a) {
+// Tiles of one KV head of sequence b (0: no rows, or another kernel's). In 64
+// bits: 2^24 tiles for each of 2^24 items are within what a call may ask for.
+template <int RT, int KT> MF_HOST_DEVICE long long paged_head_work(const PagedSeq& s, const PagedAttn& a) {
     const int rows = s.n * a.G;
     if (rows <= a.min_rows || rows > a.max_rows) return 0;
-    int w = 0;
+    long long w = 0;
     const int step = paged_step<RT>(rows);
     for (int r = 0; r < rows; r += step) w += 1 + paged_tiles<KT>(paged_span(s, a, r, step));
     return w;
@@ -109,7 +110,7 @@ MF_DEVICE long long paged_find(const PagedKv& p, const PagedAttn& a, int n, int 
     const int run = one ? 1 : (p.n_seqs + nt - 1) / nt;
     const int b0 = min((one ? lane : tid) * run, p.n_seqs), b1 = min(b0 + run, p.n_seqs);
     long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += (long long)p.n_kv_heads * paged_head_work<RT, KT>(paged_seq(p, b), a);
+    for (int b = b0; b < b1; ++b) mine += p.n_kv_heads * paged_head_work<RT, KT>(paged_seq(p, b), a);
     long long inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -153,15 +154,15 @@ MF_DEVICE long long paged_find(const PagedKv& p, const PagedAttn& a, int n, int 
     }
     for (;; ++b) {
         const PagedSeq s = paged_seq(p, b);
-        const int hw = paged_head_work<RT, KT>(s, a);
-        if (hw > 0 && at < w + (long long)hw * p.n_kv_heads) {
+        const long long hw = paged_head_work<RT, KT>(s, a);
+        if (hw > 0 && at < w + hw * p.n_kv_heads) {
             it.b = b;
             it.s = s;
             it.h = (int)paged_div(at - w, hw);
-            w += (long long)it.h * hw;
+            w += it.h * hw;
             break;
         }
-        w += (long long)hw * p.n_kv_heads;
+        w += hw * p.n_kv_heads;
     }
     it.step = paged_step<RT>(it.s.n * a.G);
     for (it.r0 = 0;; it.r0 += it.step) {
