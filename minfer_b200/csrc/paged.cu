@@ -232,6 +232,16 @@ int resident(const void* fn, int threads, size_t smem, int* blocks) {
 // Blocks per SM that the workspace of the kernels for few rows is sized for.
 int per_sm(int RT) { return RT == 16 ? 4 : 2; }
 
+// Row tiles of the chunk kernel as far as the host knows the batch: every
+// sequence begins a tile, so one of max_new tokens after the other while there
+// are as many left, then the rest in one. Without the hint all tokens are
+// taken for one sequence's, the fewest tiles: a count by equal sequences would
+// keep the one chunk among many single tokens in one share.
+long long row_tiles(int n_tokens, int G, int max_new) {
+    const long long most = max_new > 0 ? std::min(max_new, n_tokens) : n_tokens;
+    auto tiles = [&](long long n) { return (n * G + mf::PF_ROWS - 1) / mf::PF_ROWS; };
+    return n_tokens / most * tiles(most) + tiles(n_tokens % most);
+}
 // Shares of the keys in which the chunk kernel works, so that a batch of few
 // row tiles fills the SMs: the number with the shortest estimate. A CTA takes
 // about 1.9 us per tile of 128 keys and as long as three tiles to begin and
@@ -239,8 +249,8 @@ int per_sm(int RT) { return RT == 16 ? 4 : 2; }
 // (100 row tiles after 8192 keys: 3 shares, two rounds of a third each, 0.8 of
 // the time of one; 128 row tiles after 29184: one.)
 constexpr int MAX_SPLIT = 16;
-int chunk_split(int n_tokens, int n_heads, int n_kv_heads, int D, long long keys) {
-    const long long ctas = ((long long)n_tokens * (n_heads / n_kv_heads) + mf::PF_ROWS - 1) / mf::PF_ROWS * n_kv_heads;
+int chunk_split(int n_tokens, int n_heads, int n_kv_heads, int D, int max_new, long long keys) {
+    const long long ctas = row_tiles(n_tokens, n_heads / n_kv_heads, max_new) * n_kv_heads;
     const double tiles = std::max(1.0, (double)keys / mf::PF_KT), row_us = 2.0 * n_tokens * n_heads * D * 4 / 6e6;
     const int sms = num_sms();
     int best = 1;
@@ -254,9 +264,10 @@ int chunk_split(int n_tokens, int n_heads, int n_kv_heads, int D, long long keys
     }
     return best;
 }
-// Query rows x shares are bounded by the rule above (at most 4 CTAs of 256 rows per SM, or one share).
+// Query rows x shares are bounded by the rule above (at most 4 CTAs of 256 rows per SM, or one share), whatever the
+// hint: it only adds tiles.
 size_t split_bytes(int n_tokens, int n_heads, int n_kv_heads, int D) {
-    const long long ctas = ((long long)n_tokens * (n_heads / n_kv_heads) + mf::PF_ROWS - 1) / mf::PF_ROWS * n_kv_heads;
+    const long long ctas = row_tiles(n_tokens, n_heads / n_kv_heads, 0) * n_kv_heads;
     const long long n = std::min<long long>(4ll * num_sms() / ctas, MAX_SPLIT);
     return n <= 1 ? 0 : (size_t)n * n_tokens * n_heads * (D + 2) * sizeof(float);
 }
@@ -467,7 +478,7 @@ static int attention(const mf_paged_kv* kv, const mf_paged_attn_desc* d, void* s
         long long keys = (long long)p.max_pages * p.page_size;  // that a row tile sees at most
         if (d->max_len > 0) keys = std::min<long long>(keys, d->max_len);
         if (a.window > 0) keys = std::min<long long>(keys, (long long)a.window + mf::PF_ROWS / G);
-        f.n_split = chunk_split(d->n_tokens, d->n_heads, kv->n_kv_heads, D, keys);
+        f.n_split = chunk_split(d->n_tokens, d->n_heads, kv->n_kv_heads, D, d->max_new, keys);
         f.part_o = part_chunk;
         f.part_ml = (float2*)(f.part_o + f.n_split * rows * D);
         const void* fn = fa_fn(kv->dtype, D, false);
