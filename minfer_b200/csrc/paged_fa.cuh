@@ -12,7 +12,8 @@
 //                   TMEM, mask, maximum, exponentials, P as 16 bits back over
 //                   the scores. The maximum moves only when it grows by more
 //                   than 2^8 (a stale one changes rounding only, and P stays
-//                   below 2^8); then the thread rescales its row of O.
+//                   below 2^8, or 2^15: pf_lift); then the thread rescales its
+//                   row of O.
 //   warp 8          issues S_i = Q_i K^T (M128 N128) and O_i += P_i V (A = P
 //                   from TMEM, B = V as it lies in the page: the key rows are
 //                   the K extent, d is contiguous).
@@ -165,6 +166,15 @@ MF_DEVICE float2 pf_exp2_fma(f32x2 y) {
     return make_float2(__int_as_float(__float_as_int(qi.x) + (__float_as_int(ti.x) << 23)),
                        __int_as_float(__float_as_int(qi.y) + (__float_as_int(ti.y) << 23)));
 }
+
+// P = 2^(score - m + pf_lift): P is rounded to the pages' type, and fp16 holds
+// nothing below 2^-25. With the maximum m up to 2^8 behind, 2^15 is the most
+// that P may be lifted to; weights down to 2^-21 of the largest then keep fp16's
+// 11 bits and smaller ones are off by at most 2^-32 of it, so 2^20 of them by
+// at most 2^-12. (Without: 4096 keys 2^-25.5 as likely as the first were in the
+// sum but not in O.) bf16 has the exponents of a float. The factor is in
+// O and in the sum, and leaves with their quotient.
+template <typename T> constexpr float pf_lift() { return std::is_same<T, __half>::value ? 7.f : 0.f; }
 
 template <typename T> MF_DEVICE uint32_t pf_pack(float a, float b);
 template <> MF_DEVICE uint32_t pf_pack<__nv_bfloat16>(float a, float b) {
@@ -482,7 +492,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                 // P in two halves of 64 keys: the tensor core starts on the first while the second is made. One pair of
                 // every four takes its exponentials on the FMA units, since the special-function unit alone would need
                 // as long as the tensor core for the whole tile.
-                const f32x2 c2c2 = pf_two(c2, c2), bb = pf_two(-base, -base);
+                const float off = pf_lift<T>() - base;
+                const f32x2 c2c2 = pf_two(c2, c2), bb = pf_two(off, off);
                 f32x2 s2[2] = {pf_two(0.f, 0.f), pf_two(0.f, 0.f)};
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -505,8 +516,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                     } else {
 #pragma unroll
                         for (int c = 0; c < 64; c += 2) {
-                            const float e0 = ex2_approx(fmaf(__uint_as_float(sr[64 * half + c]), c2, -base));
-                            const float e1 = ex2_approx(fmaf(__uint_as_float(sr[64 * half + c + 1]), c2, -base));
+                            const float e0 = ex2_approx(fmaf(__uint_as_float(sr[64 * half + c]), c2, off));
+                            const float e1 = ex2_approx(fmaf(__uint_as_float(sr[64 * half + c + 1]), c2, off));
                             s2[c >> 1 & 1] = pf_add2(s2[c >> 1 & 1], pf_two(e0, e1));
                             pk[c >> 1] = pf_pack<T>(e0, e1);
                         }

@@ -258,6 +258,7 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                         const bool up = mx > m[mt][e] + 8.f;
                         const float mu = up ? mx : m[mt][e];
                         const float base = mu == -INFINITY ? 0.f : mu;
+                        const float off = pf_lift<T>() - base;
                         alpha[e] = up ? ex2_approx(m[mt][e] - base) : 1.f;
                         bump |= up;
                         m[mt][e] = mu;
@@ -266,7 +267,7 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                         for (int t = 0; t < KW / 8; ++t)
 #pragma unroll
                             for (int u = 0; u < 2; ++u) {
-                                const float x = ex2_approx(fmaf(s[mt][t][2 * e + u], c2, -base));
+                                const float x = ex2_approx(fmaf(s[mt][t][2 * e + u], c2, off));
                                 s[mt][t][2 * e + u] = x;
                                 sum += x;
                             }

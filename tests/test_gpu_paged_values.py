@@ -90,3 +90,29 @@ def test_scores_of_minus_infinity_weigh_nothing(dtype, seqs):
         sees = torch.arange(length - n, length, device="cuda") >= 2
         rows = out[b.start[s]:b.start[s] + n]
         assert torch.equal(rows[sees], v.expand_as(rows)[sees]) and (rows[~sees] == 0).all()
+
+
+@pytest.mark.parametrize("seqs", [[(1, 4096)] * 64, [(64, 4096)], [(300, 6000)] * 8], ids=["tokens", "chunk", "chunks"])
+def test_small_weights_of_fp16(seqs):
+    """Thousands of keys, each 2^-25.5 as likely as the first: below what fp16 holds, a 1000th of the row together.
+
+    P carries a factor 2^7, so its rounding is off by 2^-12 of P, or by 2^-25 in its subnormal range, 2^-32 of the
+    largest weight; the sum of weights is rounded nowhere near that, and v is 1: error <= n 2^-32 + 2^-11 o (the
+    output's rounding and P's) + 2^-18 o (exponentials, sums)."""
+    b = ref.Batch(seqs, 8, 2, 128, 16, F16, seed=4)
+    s0 = -17.6875  # 2^-25.52
+    for s, (n, length) in enumerate(seqs):
+        pages = b.table[s, :-(-length // 16)].long()
+        b.k[pages] = 0
+        b.k[pages, :, :, 7] = s0
+        b.v[pages] = 1
+        b.k[pages[0], :, 0, 7] = 0
+        b.v[pages[0], :, 0] = 0
+    q = torch.zeros(b.total, 8, 128, dtype=F16, device="cuda")
+    q[:, :, 7] = 1
+    out = run(b, q, scale=1.0)
+    for s, (n, length) in enumerate(seqs):
+        small = torch.arange(length - n, length, dtype=torch.float64, device="cuda") * math.exp(s0)
+        want = (small / (1 + small))[:, None, None]
+        err = (out[b.start[s]:b.start[s] + n].double() - want).abs()
+        assert (err <= length * 2.0 ** -32 + want * (2.0 ** -11 + 2.0 ** -18)).all(), (err / want).max()
