@@ -524,7 +524,12 @@ int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* desc, 
  * with a score of NaN or +inf is NaN; scores of -inf weigh nothing, alone they
  * leave the row 0.
  * max_new and max_len (0: unknown) are hints, the largest n_b and kv_lens[b]:
- * they choose between kernels, never what is computed. The workspace
+ * they choose between kernels and how the work is shared out. Results under
+ * other hints differ by rounding, and wrong hints cost time, nothing else.
+ * Scores, maxima, sums and outputs are kept in fp32. Over 16-bit pages the
+ * softmax weights are rounded to the pages' type before they meet V (by at most
+ * 2^-8 of a weight for bf16, 2^-11 or 2^-32 of the largest for fp16; their sum
+ * is not), which adds about as much error as the rounding of out. The workspace
  * (mf_paged_attention_workspace_bytes, 256-byte aligned) needs no
  * initialisation and holds nothing after the call; calls that overlap on the
  * GPU need workspaces of their own. */
