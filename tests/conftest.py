@@ -36,6 +36,12 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "slow: long-running parity case")
 
 
+def pytest_collection_modifyitems(items):
+    # What runs a program compiled from a reference checkout comes last: without one it fails, and a run that stops at
+    # its first failure has then run everything else.
+    items.sort(key=lambda item: item.path.name == "test_gpu_integration.py")
+
+
 def model_dir() -> Path:
     d = Path(os.environ.get("MF_MODEL_DIR", "/tmp/minfer_b200_models"))
     d.mkdir(parents=True, exist_ok=True)
