@@ -527,9 +527,11 @@ int mf_paged_rope_append(const mf_paged_kv* kv, const mf_paged_rope_desc* desc, 
  * they choose between kernels and how the work is shared out. Results under
  * other hints differ by rounding, and wrong hints cost time, nothing else.
  * Scores, maxima, sums and outputs are kept in fp32. Over 16-bit pages the
- * softmax weights are rounded to the pages' type before they meet V (by at most
- * 2^-8 of a weight for bf16, 2^-11 or 2^-32 of the largest for fp16; their sum
- * is not), which adds about as much error as the rounding of out. The workspace
+ * softmax weights may be rounded to the pages' type before they meet V (by at
+ * most 2^-8 of a weight for bf16, 2^-11 or 2^-32 of the largest for fp16; their
+ * sum is not), which adds about as much error as the rounding of out; the
+ * kernel for few rows keeps them to 2^-16 where a sequence has up to 8 (new
+ * tokens x heads of a group). The workspace
  * (mf_paged_attention_workspace_bytes, 256-byte aligned) needs no
  * initialisation and holds nothing after the call; calls that overlap on the
  * GPU need workspaces of their own. */

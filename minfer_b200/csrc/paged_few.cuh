@@ -60,6 +60,10 @@ template <> MF_DEVICE void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+template <typename T> MF_DEVICE float2 pw_unpack(uint32_t v);
+template <> MF_DEVICE float2 pw_unpack<__nv_bfloat16>(uint32_t v) { return make_float2(bf16_lo(v), bf16_hi(v)); }
+template <> MF_DEVICE float2 pw_unpack<__half>(uint32_t v) { return f16x2_to_f2(v); }
+
 // MT: 16-row tiles of query rows (RT = 16 MT).
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(PW_THREADS, 2)
@@ -146,13 +150,19 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
             if (j1 <= 0) break;  // only the item's first unit is in this range
             const int rows = min(it.step, it.s.n * a.G - it.r0);
             const int key0 = it.k.lo / KT * KT;
+            // Rows r and r + 8 of a 16-row tile are one thread's. An item of up to 8 rows has each in both places, and P
+            // rounded to the pages' type in the first and what that left of it in the second: the products are the same in
+            // number, and the two halves of O, added at the end, hold P exact to 2^-16 (fp16: 2^-22). (For more rows the second
+            // part would be as many products again: 32 rows of 64 x 4 tokens at 4096 keys 245 us in place of 222.)
+            const bool twice = rows <= 8;
+            auto row_at = [&](int r) { return min(twice ? r & 7 : r, rows - 1); };  // rows past the end repeat the last
             const T* qb = reinterpret_cast<const T*>(a.q) + (long long)it.s.row * a.q_stride + (long long)it.h * a.G * D;
             auto q_row = [&](int r) { return qb + (long long)((it.r0 + r) / a.G) * a.q_stride + (long long)((it.r0 + r) % a.G) * D; };
             uint32_t qf[MT == 1 ? D / 16 : 1][4];
             if constexpr (MT == 1) {
                 const int r = lane >> 2, c = (lane & 3) * 2;
-                const T* q0 = q_row(min(r, rows - 1));
-                const T* q1 = q_row(min(r + 8, rows - 1));
+                const T* q0 = q_row(row_at(r));
+                const T* q1 = q_row(row_at(r + 8));
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     qf[k][0] = *reinterpret_cast<const uint32_t*>(q0 + 16 * k + c) ^ flip;
@@ -164,20 +174,20 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                 named_bar_sync(1, PW_WARPS * 32);  // the last item's rows are done with
                 for (int e = threadIdx.x; e < RT * (D / 8); e += PW_WARPS * 32) {
                     const int r = e / (D / 8), cc = e % (D / 8);
-                    uint4 v = *reinterpret_cast<const uint4*>(q_row(min(r, rows - 1)) + cc * 8);
+                    uint4 v = *reinterpret_cast<const uint4*>(q_row(row_at(r)) + cc * 8);
                     v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
                     *reinterpret_cast<uint4*>(q_s + r * (D * 2) + ((cc ^ (r & 7)) << 4)) = v;
                 }
                 named_bar_sync(1, PW_WARPS * 32);
             }
-            // this lane's rows: lane / 4 (+ 8) of each 16-row tile; rows past the end repeat the last and are not stored
+            // this lane's rows: lane / 4 (+ 8) of each 16-row tile; repeated ones are not stored
             int pos[MT][2], lo[MT][2];
             int hi_all = 0x7fffffff, lo_all = 0;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    pos[mt][e] = it.s.first + (it.r0 + min(16 * mt + 8 * e + (lane >> 2), rows - 1)) / a.G;
+                    pos[mt][e] = it.s.first + (it.r0 + row_at(16 * mt + 8 * e + (lane >> 2))) / a.G;
                     lo[mt][e] = a.window > 0 ? pos[mt][e] - a.window + 1 : 0;
                     hi_all = min(hi_all, pos[mt][e]);
                     lo_all = max(lo_all, lo[mt][e]);
@@ -285,8 +295,15 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
 #pragma unroll
                     for (int kk = 0; kk < KW / 16; ++kk) {
                         pa[mt][kk][0] = pf_pack<T>(s[mt][2 * kk][0], s[mt][2 * kk][1]);
-                        pa[mt][kk][1] = pf_pack<T>(s[mt][2 * kk][2], s[mt][2 * kk][3]);
                         pa[mt][kk][2] = pf_pack<T>(s[mt][2 * kk + 1][0], s[mt][2 * kk + 1][1]);
+                        if (twice) {
+                            const float2 h0 = pw_unpack<T>(pa[mt][kk][0]), h1 = pw_unpack<T>(pa[mt][kk][2]);
+                            s[mt][2 * kk][2] -= h0.x;
+                            s[mt][2 * kk][3] -= h0.y;
+                            s[mt][2 * kk + 1][2] -= h1.x;
+                            s[mt][2 * kk + 1][3] -= h1.y;
+                        }
+                        pa[mt][kk][1] = pf_pack<T>(s[mt][2 * kk][2], s[mt][2 * kk][3]);
                         pa[mt][kk][3] = pf_pack<T>(s[mt][2 * kk + 1][2], s[mt][2 * kk + 1][3]);
                     }
                 }
@@ -328,6 +345,13 @@ __global__ void __launch_bounds__(PW_THREADS, 2)
                 if (lane == 0) mbar_arrive(&free_[st]);
             }
 
+            if (twice) {
+#pragma unroll
+                for (int d = 0; d < D / 8; ++d) {
+                    o[0][d][0] += o[0][d][2];
+                    o[0][d][1] += o[0][d][3];
+                }
+            }
             // join the four warps' parts, PW_COLS columns at a time
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)

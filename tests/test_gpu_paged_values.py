@@ -116,3 +116,27 @@ def test_small_weights_of_fp16(seqs):
         want = (small / (1 + small))[:, None, None]
         err = (out[b.start[s]:b.start[s] + n].double() - want).abs()
         assert (err <= length * 2.0 ** -32 + want * (2.0 ** -11 + 2.0 ** -18)).all(), (err / want).max()
+
+
+class WithAbsoluteValues:
+    """A batch whose V is |V|: its attention is sum p |v|."""
+
+    def __init__(self, b):
+        self.__dict__ = {**b.__dict__, "v": b.v.abs()}
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("heads", [(32, 8), (8, 8), (5, 1), (8, 1)], ids=str)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("max_new", [0, 1], ids=["", "hint"])
+def test_decode_rounds_only_its_output(dtype, heads, d, max_new):
+    """Up to 8 rows: P is kept in two parts, so where the reference's bound allows twice a rounding of P to the pages'
+    type (2 u sum p |v|), two roundings of its second part are all that is left: the first leaves at most 2^-8 P, the
+    second 2^-8 of that (fp16: less), 2^-15 sum p |v| for both."""
+    b = ref.Batch([(1, n) for n in (1, 17, 300, 4096, 9000, 2500)], *heads, d, 16, dtype, seed=6)
+    q = b.q()
+    out = run(b, q, max_new=max_new).double()
+    want, bound = ref.attention(b, q)
+    a = ref.attention(WithAbsoluteValues(b), q)[0]
+    bound = bound + a * (2.0 ** -15 - torch.finfo(dtype).eps)
+    assert ((out - want).abs() <= bound).all()
