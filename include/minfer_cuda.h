@@ -590,7 +590,8 @@ int mf_sample_step(const int* cand_ids, const float* cand_vals, int top_k, float
  * the first maximum. Any top_k. Each candidate's weight is rounded to 2^-45 of
  * the largest, so a candidate 32 or more below the top counts as nothing in a
  * sum, and a target that falls within that of a border may take the border's
- * other side. The result does not depend on the launch. probs (optional) receives the
+ * other side. The result does not depend on the launch. No presence penalty (it
+ * changes the logits, before this call). probs (optional) receives the
  * id's probability under the last softmax (1 for temp <= 0). A row without any
  * value above -inf gives id -1 and probability 0. vocab is at most 2^18. */
 int mf_sample_batch(int* ids, float* probs, const void* logits, int dtype, long long ld, int n_rows, int vocab,

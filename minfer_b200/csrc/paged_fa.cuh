@@ -32,9 +32,12 @@
 // core and as many of the special-function unit (1536 with a quarter of the
 // exponentials on the FMA units). A tile's softmax (2200 cycles) and its MMAs
 // with their barriers (1200) follow each other, so a pair takes about 3450.
-// Measured: 4096 x 4096 causal, 32/8 heads, 142-162 us (0.52-0.59 of the cuBLAS
-// bf16 rate, diagonal tiles counted by their halves); 512 tokens after 28672,
-// 64/8 heads, 451-472 us (1.03-1.08 PFLOP/s on the 128 SMs that have a tile).
+// Measured: 4096 x 4096 causal, 32/8 heads, 142 us at 1965 MHz and 163 in a long
+// loop, where the power cap takes the clock to 1750 (0.59 and 0.51 of the cuBLAS
+// bf16 rate, diagonal tiles counted by their halves); of the 142 the pairs take
+// 100 and the CTAs' beginnings, ends and last round the rest. 512 tokens after
+// 28672, 64/8 heads, 413-440 and 478 us (1.10-1.18 and 1.02 PFLOP/s on the 128
+// SMs that have a tile).
 // Slower: two buffers of 64-key scores (159 / 513 us: an MMA of 64 keys takes
 // 55 cycles, not 32), four groups of 64 columns (158 / 444), exponentials before
 // the maximum is known (154 / 470).

@@ -16,9 +16,9 @@
 // in the chunk kernel the maximum moves only when it grows by more than 2^8;
 // runs that no row sees are not read, and of a run that is seen in part the
 // other rows are masked (scores) and zeroed (V, in registers).
-// Measured: 32 sequences to 32768 keys, 64/8 heads, 348 us (2.28 GB, at the copy
-// rate); 64 sequences to 2048 keys, 16 heads of 64, 56 us (0.69); one sequence
-// of 4096 keys 14 us with the join, a chain of latencies.
+// Measured: 32 sequences to 32768 keys, 64/8 heads, 354 us (2.28 GB, 0.98 of the
+// copy rate); 64 sequences to 2048 keys, 16 heads of 64, 57 us (0.68); one
+// sequence of 4096 keys 14 us with the join, a chain of latencies.
 #pragma once
 
 #include "paged_fa.cuh"

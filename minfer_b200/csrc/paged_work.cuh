@@ -38,9 +38,11 @@ struct PagedAttn {
 constexpr float PAGED_GAVE_UP = -1.f;
 
 // A kernel for few rows that follows a chunk kernel of the same call works on
-// other rows, so it starts as that kernel's CTAs leave the SMs and waits for it
-// only at its own end (whoever waits for this one then waits for both). What
-// both read was there before: the chunk kernel lets this one start only after
+// other rows, so it starts on SMs that that kernel's CTAs leave or never had and
+// waits for it only at its own end (whoever waits for this one then waits for
+// both). Each CTA keeps its place until then: beside a chunk kernel that still
+// runs only as many work as fit the free SMs at once, the others follow it.
+// What both read was there before: the chunk kernel lets this one start only after
 // its own wait.
 MF_DEVICE void paged_begin(const PagedAttn& a) {
     if (!a.beside) pdl_wait();

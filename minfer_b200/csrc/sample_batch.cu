@@ -34,7 +34,7 @@ int sample_batch(int* ids, float* probs, const void* logits, int dtype, long lon
         (((uintptr_t)ids | (uintptr_t)probs | (uintptr_t)draws | (uintptr_t)temp | (uintptr_t)top_k | (uintptr_t)top_p |
           (uintptr_t)min_p) & 3) != 0)
         return fail(MF_E_INVALID, "misaligned argument");
-    // Blocks per row: as many as keep a block's slice at 4096 logits or more, at most 8.
+    // Blocks per row: as few as keep a block's slice at 4096 logits or fewer, at most 8.
     int cluster = 1;
     while (cluster < mf::SB_MAX_CLUSTER && (vocab + cluster - 1) / cluster > 4096) cluster *= 2;
     if ((long long)n_rows * cluster > 0x7fffffffll) return fail(MF_E_UNSUPPORTED, "too many rows");

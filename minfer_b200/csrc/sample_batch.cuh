@@ -28,9 +28,9 @@
 // off by at most 2^-46 per term. In floats a vocabulary of 10^5 would move the
 // border of every hundredth draw.
 //
-// Measured, 151936 fp32 logits: one row 15 us with top_k 50, 46 with top_p 0.9
-// alone; 64 rows 41 and 125 us (the floor, one read, is 6; the maximum alone
-// takes 13). Bound by latencies (an exchange over the cluster is about a
+// Measured, 151936 fp32 logits, times per call: one row 16 us with top_k 50, 48
+// with top_p 0.9 alone; 64 rows 47 and 129 us (the floor, one read, is 6; the
+// maximum alone takes 18, of one row 7.5). Bound by latencies (an exchange over the cluster is about a
 // microsecond, and there are five to nine) and, without top_k, by shared-memory
 // atomics and 64-bit arithmetic. Exact bins took three atomics per logit more
 // (147 us for a mixed batch of 64 rows, now 79), a bitonic sort of the
@@ -47,7 +47,7 @@ constexpr int SB_BINS = 512;        // one per thread
 constexpr int SB_LIST = 64;         // candidates left to one warp (two per lane)
 constexpr int SB_FEW = 2048;        // candidates that one block orders: four per thread
 constexpr int SB_MAX_CLUSTER = 8;
-constexpr int SB_MAX_VOCAB = 1 << 18;  // 2^18 weights of at most 2^45: sums below 2^63
+constexpr int SB_MAX_VOCAB = 1 << 18;  // 2^18 weights of at most 2^45: sums of at most 2^63, unsigned
 constexpr double SB_ONE = 35184372088832.0;  // 2^45
 
 struct SampleBatch {
