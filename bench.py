@@ -16,8 +16,8 @@ Each step reads ~16.4 GB (weights + KV), far more than L2, so no flush is
 needed between steps.
 
 `--impl reference` runs the reference's own CPU token loop (oracle/_ref, built
-from the reference sources; the oracle port if absent) on the host cores on a
-bounded sample of the same workload.
+from the reference sources) on the host cores on a bounded sample of the same
+workload; without that build it says "unavailable" and measures nothing.
 Multi-GPU runs (torchrun, one rank per GPU) decode the same single stream
 with tensor parallelism over the N GPUs (strong scaling): each rank holds a
 1/N shard of every projection, the two all-reduces per layer are fused into
@@ -533,6 +533,11 @@ def main():
 
     if args.impl == "reference":
         if rank != 0:
+            return
+        from oracle import oracle_py
+
+        if not oracle_py.ref_available():  # the oracle's restatement is not the reference
+            print(json.dumps({"impl": "reference", "unavailable": "oracle/_ref is not built: no reference checkout here"}), flush=True)
             return
         path, _ = prepare_model(args.workload, 0, 1)
         thr = host_threads()
